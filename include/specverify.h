@@ -42,6 +42,10 @@
  *                         diffspec/draft/diffspec_model.py:620-624 (root prepend)
  *   tv_chunk_select,
  *   tv_gather_rows        diffspec/draft/draft_network.py:1514-1612 (retrieval)
+ *   tv_residual_accept    no counterpart (diffspec/draft/tree_verification.py:100-162
+ *                         samples and matches)
+ *   tv_add_rms_norm       diffspec/runtime/llama_target_model.py:124-138 (LlamaRMSNorm)
+ *                         with the residual's addition before it
  */
 #ifndef SPECVERIFY_H_
 #define SPECVERIFY_H_
@@ -302,6 +306,60 @@ typedef struct tv_accept_args {
 int tv_accept_workspace_size(const tv_accept_args* args, size_t* bytes);
 int tv_accept(const tv_accept_args* args, void* stream);
 
+/* Acceptance by the residual rule, from given uniform numbers: the tokens are
+ * distributed as the target's own samples whatever the draft proposed (tv_accept
+ * mode 1 samples one token per node and matches drafts against it instead).
+ * Per sequence b, with p = softmax(logits[b, node] / temperature), the children
+ * of a node are tried in index order:
+ *   probs == NULL (fixed drafts, e.g. the top-k of the draft's distribution):
+ *     child i is accepted when uniform[i] * (1 - removed) < p(draft[i]); a
+ *     rejected token leaves p (removed += p of it); a second child with the
+ *     same token is never accepted;
+ *   probs (sampled drafts: node's children drawn independently from
+ *     q = probs[b, node]): the distribution after rejections is (p - a q)+ / s,
+ *     a = 0, s = 1 at first, then a += s, s = sum (p - a q)+; child i is
+ *     accepted when uniform[i] * s * q(draft[i]) < (p(draft[i]) - a q(draft[i]))+.
+ * The walk goes on at the accepted child.  Where none is accepted the next
+ * token is the first word at which the cumulated weight of what is left
+ * exceeds uniform[0] * its sum (of p itself where nothing is left).
+ * Sums and comparisons are in 64 bits; there are no atomics on values, so the
+ * same inputs give the same result.
+ *
+ * parent / draft as tv_accept (parent -1: child of the root), and every parent
+ * comes before its children.  counts (optional): sequence b has counts[b]
+ * nodes, 1 <= counts[b] <= rows; what lies behind them is not read.
+ * result [batch][8 + 2 rows] as tv_accept's result, unused path entries -1;
+ * next_tokens [batch][rows]: the drawn token at the last accepted node, -1
+ * elsewhere.  A sequence with a bad parent, draft token or count, or whose
+ * walk ends at a row that is no distribution (no finite logit, a NaN, +inf),
+ * gets result[0] = TV_ERR_INPUT, a path of length 0 and token -1.
+ * rows <= 1024.  workspace: tv_residual_accept_workspace_size bytes, 16-byte
+ * aligned. */
+typedef struct tv_residual_accept_args {
+  int32_t logits_dtype;          /* TV_BF16, TV_F16 or TV_F32               */
+  int32_t batch, rows, vocab;
+  const void* logits;            /* [batch][rows][vocab], unit stride on vocab */
+  int64_t logits_sb, logits_sm;
+  const int64_t* draft;          /* [batch][rows]                           */
+  int64_t draft_sb;
+  const int64_t* parent;         /* [batch][rows - 1]                       */
+  int64_t parent_sb;
+  const int32_t* counts;         /* optional [batch]                        */
+  const float* uniform;          /* [batch][rows] in [0, 1)                 */
+  int64_t uniform_sb;
+  int32_t probs_dtype;
+  const void* probs;             /* optional [batch][rows][vocab]           */
+  int64_t probs_sb, probs_sm;
+  float temperature;
+  int64_t* next_tokens;
+  int64_t* result;
+  void* workspace;
+  size_t workspace_bytes;
+} tv_residual_accept_args;
+
+int tv_residual_accept_workspace_size(const tv_residual_accept_args* args, size_t* bytes);
+int tv_residual_accept(const tv_residual_accept_args* args, void* stream);
+
 /* ---- compaction -------------------------------------------------------
  * Contiguous cache: for every slice s < num_slices of `data`
  * (slice base = data + s * slice_stride_bytes, row r at
@@ -512,6 +570,22 @@ int tv_rms_norm(const void* x, int64_t x_row_stride, const void* weight, void* y
                 int32_t rows, int32_t cols, float eps, int32_t dtype, void* stream);
 int tv_silu_mul(const void* gate, const void* up, int64_t in_row_stride, void* out, int64_t out_row_stride,
                 int32_t rows, int32_t cols, int32_t dtype, void* stream);
+
+/* The residual's addition and the LlamaRMSNorm after it
+ * (runtime/llama_target_model.py:124-138) in one pass, per row r:
+ *   h = T(x + residual)  -> residual_out (may be residual itself);
+ *   y_scale == NULL: y = T(T(h * inv) * weight), inv = 1 / sqrt(mean(h^2) + eps),
+ *     the roundings of tv_rms_norm (y may be x itself);
+ *   y_scale != NULL: y is e4m3 (one byte an element, y_row_stride in elements):
+ *     f = h * inv * weight in fp32, y_scale[r] = max|f| / 448,
+ *     y = e4m3(f / y_scale[r]).  A row of zeros has scale 0; a row with a NaN
+ *     has scale NaN and NaN throughout.
+ * Any cols >= 1, strides and alignment (rows of 16-byte multiples at 16-byte
+ * aligned addresses are read as vectors).  rows == 0 does nothing. */
+int tv_add_rms_norm(const void* x, int64_t x_row_stride, const void* residual, int64_t residual_row_stride,
+                    const void* weight, void* residual_out, int64_t residual_out_row_stride, void* y,
+                    int64_t y_row_stride, float* y_scale, int32_t rows, int32_t cols, float eps, int32_t dtype,
+                    void* stream);
 
 #ifdef __cplusplus
 }

@@ -7,6 +7,11 @@
 // One CTA per row for the norm (the row's sum of squares is a block
 // reduction); the gate is a flat grid over 8-element chunks.  Rows are read
 // as 16-byte vectors: columns a multiple of 8, rows 16-byte aligned.
+//
+// tv_add_rms_norm takes the residual's addition in front of the norm into the
+// same pass and can hand the row on in 8 bits with its scale.
+#include <cuda_fp8.h>
+
 #include "common.cuh"
 #include "specverify.h"
 
@@ -86,6 +91,243 @@ __global__ void silu_mul_kernel(const T* __restrict__ g, const T* __restrict__ u
   }
 }
 
+// ---- residual addition + RMSNorm ---------------------------------------------
+//
+//   h = T(x + r),  y = T(T(h * inv) * w),  inv = 1 / sqrt(mean(h^2) + eps)
+// or, in 8 bits,
+//   f = h * inv * w (fp32),  s = max|f| / 448,  y = e4m3(f / s).
+//
+// The norm is of the stored (rounded) stream h, so a later reader of h sees
+// the row that was normalised; the 16-bit output rounds as tv_rms_norm does.
+// One CTA per row.  A thread keeps its NC chunks of VEC elements of h in
+// registers between the two passes, so every input is read once and every
+// output written once: the kernel is bound by HBM for many rows and by
+// latency (two or three block reductions) for few.
+template <typename T, int VEC> struct Chunk;
+template <typename T> struct Chunk<T, 8> {
+  uint4 v;
+  __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = v; }
+  __device__ __forceinline__ void get(float* f) const { unpack8<T>(v, f); }
+  __device__ __forceinline__ void set(const float* f) { v = pack8<T>(f); }
+};
+template <typename T> struct Chunk<T, 1> {
+  T v;
+  __device__ __forceinline__ void load(const T* p) { v = *p; }
+  __device__ __forceinline__ void store(T* p) const { *p = v; }
+  __device__ __forceinline__ void get(float* f) const { f[0] = Elem<T>::to_f(v); }
+  __device__ __forceinline__ void set(const float* f) { v = Elem<T>::from_f(f[0]); }
+};
+
+// Maximum that keeps a NaN of either side (fmaxf drops it).
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+template <int VEC>
+__device__ __forceinline__ void store_e4m3(uint8_t* p, const float* f) {
+  if constexpr (VEC == 8) {
+    uint2 u;
+    __nv_fp8x2_storage_t* e = reinterpret_cast<__nv_fp8x2_storage_t*>(&u);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      e[k] = __nv_cvt_float2_to_fp8x2(make_float2(f[2 * k], f[2 * k + 1]), __NV_SATFINITE, __NV_E4M3);
+    *reinterpret_cast<uint2*>(p) = u;
+  } else {
+    *p = __nv_cvt_float_to_fp8(f[0], __NV_SATFINITE, __NV_E4M3);
+  }
+}
+
+struct AddNormArgs {
+  const void* x;
+  const void* r;
+  const void* w;
+  void* h;
+  void* y;
+  float* scale;
+  int64_t xs, rs, hs, ys;
+  int cols;
+  float eps;
+};
+
+// NC chunks per thread stay in registers; WIDE rows (more than that) are read
+// back from h, each thread its own chunks.
+template <typename T, bool FP8, int VEC, int NC, bool WIDE>
+__global__ void __launch_bounds__(512) add_rms_norm_kernel(const AddNormArgs a) {
+  const T* x = static_cast<const T*>(a.x) + (int64_t)blockIdx.x * a.xs;
+  const T* r = static_cast<const T*>(a.r) + (int64_t)blockIdx.x * a.rs;
+  const T* w = static_cast<const T*>(a.w);
+  T* h = static_cast<T*>(a.h) + (int64_t)blockIdx.x * a.hs;
+  const int step = blockDim.x * VEC;
+  const int first = threadIdx.x * VEC;
+  Chunk<T, VEC> keep[NC];
+  float ss = 0.f;
+  if (!WIDE) {
+    Chunk<T, VEC> cr[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      if (first + i * step < a.cols) {
+        keep[i].load(x + first + i * step);
+        cr[i].load(r + first + i * step);
+      }
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      if (first + i * step < a.cols) {
+        float f[VEC], g[VEC];
+        keep[i].get(f);
+        cr[i].get(g);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) f[k] += g[k];
+        keep[i].set(f);
+        keep[i].store(h + first + i * step);
+        keep[i].get(f);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) ss = fmaf(f[k], f[k], ss);
+      }
+  } else {
+    for (int c = first; c < a.cols; c += step) {
+      Chunk<T, VEC> u, v;
+      float f[VEC], g[VEC];
+      u.load(x + c);
+      v.load(r + c);
+      u.get(f);
+      v.get(g);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) f[k] += g[k];
+      u.set(f);
+      u.store(h + c);
+      u.get(f);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) ss = fmaf(f[k], f[k], ss);
+    }
+  }
+  __shared__ float part[16];
+  __shared__ float part_max[16];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  if (lane == 0) part[warp] = ss;
+  __syncthreads();
+  float tot = 0.f;
+  for (int i = 0; i < warps; ++i) tot += part[i];
+  const float inv = rsqrtf(tot / (float)a.cols + a.eps);
+
+  if constexpr (!FP8) {
+    T* y = static_cast<T*>(a.y) + (int64_t)blockIdx.x * a.ys;
+    auto put = [&](const Chunk<T, VEC>& u, int c) {
+      Chunk<T, VEC> v;
+      float f[VEC], g[VEC];
+      v.load(w + c);
+      u.get(f);
+      v.get(g);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) f[k] = round_to<T>(f[k] * inv) * g[k];
+      v.set(f);
+      v.store(y + c);
+    };
+    if (!WIDE) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        if (first + i * step < a.cols) put(keep[i], first + i * step);
+    } else {
+      for (int c = first; c < a.cols; c += step) {
+        Chunk<T, VEC> u;
+        u.load(h + c);
+        put(u, c);
+      }
+    }
+  } else {
+    uint8_t* y = static_cast<uint8_t*>(a.y) + (int64_t)blockIdx.x * a.ys;
+    auto row = [&](const Chunk<T, VEC>& u, int c, float* f) {
+      Chunk<T, VEC> v;
+      float g[VEC];
+      v.load(w + c);
+      u.get(f);
+      v.get(g);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) f[k] = f[k] * inv * g[k];
+    };
+    float mx = 0.f;
+    auto top = [&](const Chunk<T, VEC>& u, int c) {
+      float f[VEC];
+      row(u, c, f);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) mx = max_nan(mx, fabsf(f[k]));
+    };
+    if (!WIDE) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        if (first + i * step < a.cols) top(keep[i], first + i * step);
+    } else {
+      for (int c = first; c < a.cols; c += step) {
+        Chunk<T, VEC> u;
+        u.load(h + c);
+        top(u, c);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    if (lane == 0) part_max[warp] = mx;
+    __syncthreads();
+    mx = part_max[0];
+    for (int i = 1; i < warps; ++i) mx = max_nan(mx, part_max[i]);
+    const float s = mx * (1.0f / 448.0f);
+    if (threadIdx.x == 0) a.scale[blockIdx.x] = s;
+    // A row of zeros has scale 0 and stays zero.  The reciprocal of a scale
+    // below 2^-100 is not safe to multiply with: divide there.
+    const bool tiny = s < 7.8886091e-31f;
+    const float is = 1.0f / s;
+    auto put = [&](const Chunk<T, VEC>& u, int c) {
+      float f[VEC];
+      row(u, c, f);
+      if (tiny) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) f[k] = s == 0.f ? 0.f : f[k] / s;
+      } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) f[k] *= is;
+      }
+      store_e4m3<VEC>(y + c, f);
+    };
+    if (!WIDE) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        if (first + i * step < a.cols) put(keep[i], first + i * step);
+    } else {
+      for (int c = first; c < a.cols; c += step) {
+        Chunk<T, VEC> u;
+        u.load(h + c);
+        put(u, c);
+      }
+    }
+  }
+}
+
+template <typename T, bool FP8, int VEC, int NC, bool WIDE>
+int launch_add_norm(const AddNormArgs& a, int rows, int threads, cudaStream_t st) {
+  add_rms_norm_kernel<T, FP8, VEC, NC, WIDE><<<rows, threads, 0, st>>>(a);
+  return check_launch();
+}
+
+// Threads per row: enough that a row's chunks fit NC registers' worth, at most
+// 512 (a row of more than 512 * NC chunks is read back from h).
+template <typename T, bool FP8>
+int pick_add_norm(const AddNormArgs& a, int rows, bool vec, cudaStream_t st) {
+  const int chunks = vec ? a.cols / 8 : a.cols;
+  auto fit = [&](int nc) { return ((chunks + nc - 1) / nc + 31) / 32 * 32; };
+  if (vec) {
+    if (fit(1) <= 512) return launch_add_norm<T, FP8, 8, 1, false>(a, rows, fit(1), st);
+    if (fit(2) <= 512) return launch_add_norm<T, FP8, 8, 2, false>(a, rows, fit(2), st);
+    if (fit(4) <= 512) return launch_add_norm<T, FP8, 8, 4, false>(a, rows, fit(4), st);
+    return launch_add_norm<T, FP8, 8, 1, true>(a, rows, 512, st);
+  }
+  if (fit(4) <= 512) return launch_add_norm<T, FP8, 1, 4, false>(a, rows, fit(4), st);
+  if (fit(16) <= 512) return launch_add_norm<T, FP8, 1, 16, false>(a, rows, fit(16), st);
+  return launch_add_norm<T, FP8, 1, 1, true>(a, rows, 512, st);
+}
+
 bool vec_ok(const void* p, int64_t stride) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (stride % 8) == 0;
 }
@@ -114,6 +356,27 @@ int tv_rms_norm(const void* x, int64_t x_row_stride, const void* weight, void* y
                                                            static_cast<const __half*>(weight),
                                                            static_cast<__half*>(y), y_row_stride, cols, eps);
   return check_launch();
+}
+
+int tv_add_rms_norm(const void* x, int64_t x_row_stride, const void* residual, int64_t residual_row_stride,
+                    const void* weight, void* residual_out, int64_t residual_out_row_stride, void* y,
+                    int64_t y_row_stride, float* y_scale, int32_t rows, int32_t cols, float eps, int32_t dtype,
+                    void* stream) {
+  if (rows < 0 || cols <= 0) return TV_ERR_SHAPE;
+  if (dtype != TV_BF16 && dtype != TV_F16) return TV_ERR_DTYPE;
+  if (rows == 0) return TV_OK;
+  if (!x || !residual || !weight || !residual_out || !y) return TV_ERR_NULL;
+  AddNormArgs a{x, residual, weight, residual_out, y, y_scale, x_row_stride, residual_row_stride,
+                residual_out_row_stride, y_row_stride, cols, eps};
+  const bool y_ok = y_scale ? (reinterpret_cast<uintptr_t>(y) & 7) == 0 && (y_row_stride % 8) == 0
+                            : vec_ok(y, y_row_stride);
+  const bool vec = (cols % 8) == 0 && vec_ok(x, x_row_stride) && vec_ok(residual, residual_row_stride) &&
+                   vec_ok(weight, 0) && vec_ok(residual_out, residual_out_row_stride) && y_ok;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == TV_BF16)
+    return y_scale ? pick_add_norm<__nv_bfloat16, true>(a, rows, vec, st)
+                   : pick_add_norm<__nv_bfloat16, false>(a, rows, vec, st);
+  return y_scale ? pick_add_norm<__half, true>(a, rows, vec, st) : pick_add_norm<__half, false>(a, rows, vec, st);
 }
 
 int tv_silu_mul(const void* gate, const void* up, int64_t in_row_stride, void* out, int64_t out_row_stride,

@@ -98,6 +98,19 @@ class LmheadArgs(ctypes.Structure):
     ]
 
 
+class ResidualAcceptArgs(ctypes.Structure):
+    """Mirror of ``tv_residual_accept_args``."""
+    _fields_ = [
+        ("logits_dtype", c_i32), ("batch", c_i32), ("rows", c_i32), ("vocab", c_i32),
+        ("logits", c_vp), ("logits_sb", c_i64), ("logits_sm", c_i64),
+        ("draft", c_vp), ("draft_sb", c_i64), ("parent", c_vp), ("parent_sb", c_i64),
+        ("counts", c_vp), ("uniform", c_vp), ("uniform_sb", c_i64),
+        ("probs_dtype", c_i32), ("probs", c_vp), ("probs_sb", c_i64), ("probs_sm", c_i64),
+        ("temperature", c_f32), ("next_tokens", c_vp), ("result", c_vp),
+        ("workspace", c_vp), ("workspace_bytes", c_size),
+    ]
+
+
 # name -> (restype, argtypes)
 _SIGNATURES = {
     "tv_status_string": (ctypes.c_char_p, [c_i32]),
@@ -115,6 +128,8 @@ _SIGNATURES = {
     "tv_mask_word_summary": (c_i32, [c_vp, c_i32, c_i32, c_i32, c_i64, c_i64, c_vp, c_i64, c_vp]),
     "tv_accept_workspace_size": (c_i32, [ctypes.POINTER(AcceptArgs), ctypes.POINTER(c_size)]),
     "tv_accept": (c_i32, [ctypes.POINTER(AcceptArgs), c_vp]),
+    "tv_residual_accept_workspace_size": (c_i32, [ctypes.POINTER(ResidualAcceptArgs), ctypes.POINTER(c_size)]),
+    "tv_residual_accept": (c_i32, [ctypes.POINTER(ResidualAcceptArgs), c_vp]),
     "tv_compact_contig": (c_i32, [c_vp, c_i64, c_i64, c_i64, c_i32, c_i64, c_vp, c_i32, c_vp]),
     "tv_copy_pages": (c_i32, [c_vp, c_i32, c_i64, c_i64, c_i64, c_vp, c_i32, c_i32, c_vp]),
     "tv_compact_paged": (c_i32, [c_vp, c_i32, c_i32, c_i64, c_i64, c_i64, c_i64, c_i32, c_i32, c_vp, c_vp,
@@ -132,6 +147,8 @@ _SIGNATURES = {
                                 c_vp, c_vp]),
     "tv_gather_rows": (c_i32, [c_i32, c_i32, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i32, c_vp, c_vp, c_i64, c_vp]),
     "tv_rms_norm": (c_i32, [c_vp, c_i64, c_vp, c_vp, c_i64, c_i32, c_i32, c_f32, c_i32, c_vp]),
+    "tv_add_rms_norm": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_i32, c_i32, c_f32,
+                                c_i32, c_vp]),
     "tv_silu_mul": (c_i32, [c_vp, c_vp, c_i64, c_vp, c_i64, c_i32, c_i32, c_i32, c_vp]),
 }
 
@@ -199,6 +216,16 @@ def dtype_code(dtype: torch.dtype) -> int:
 
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def launch(dev: torch.device, fn, *args) -> int:
+    """``fn(*args, stream)`` on ``dev``'s current stream, with ``dev`` current
+    for the call (a kernel launches on the current device, not its tensors')."""
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    if dev.index == torch.cuda.current_device():
+        return fn(*args, stream)
+    with torch.cuda.device(dev):
+        return fn(*args, stream)
 
 
 def ptr(t) -> int:

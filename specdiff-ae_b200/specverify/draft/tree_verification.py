@@ -32,8 +32,8 @@ import torch
 from .. import _lib
 from ..core.bundle_scheduler import BundleScheduler
 
-__all__ = ["prepare_logits_processor", "tree_decoding", "verify", "verify_new", "accept", "compact_kv",
-           "AcceptResult"]
+__all__ = ["prepare_logits_processor", "tree_decoding", "verify", "verify_new", "accept", "accept_residual",
+           "compact_kv", "AcceptResult"]
 
 MODE_GREEDY, MODE_SAMPLE, MODE_GIVEN = 0, 1, 2
 RESULT_HEADER = 8
@@ -96,11 +96,21 @@ class AcceptResult:
             res[RESULT_HEADER + rows:RESULT_HEADER + rows + len(tokens)] = torch.tensor(tokens, dtype=torch.int64)
         return cls(torch.zeros(rows, dtype=torch.int64, device=device), res.to(device), rows)
 
+    def sequence(self, b: int) -> "AcceptResult":
+        """Sequence ``b`` of a batched result (:func:`accept_residual`)."""
+        return AcceptResult(self.next_tokens[b], self.result[b], self.rows)
+
     def to_host(self):
-        """One D2H copy; returns a dict with python ints / lists."""
-        h = self.result.cpu().tolist()
+        """One D2H copy; returns a dict with python ints / lists (a list of
+        them, one per sequence, for a batched result)."""
+        if self.result.dim() == 2:
+            return [self._parse(h) for h in self.result.cpu().tolist()]
+        return self._parse(self.result.cpu().tolist())
+
+    def _parse(self, h: list) -> dict:
         if h[0] != 0:
-            raise _lib.SpecVerifyError(h[0], "tv_accept: parent pointers out of range or cyclic")
+            raise _lib.SpecVerifyError(h[0], "tv_accept: parent pointers out of range or cyclic, or (residual rule) "
+                                             "a bad draft token, node count or row of logits")
         n = h[2]
         return {
             "max_id": h[1],
@@ -168,6 +178,77 @@ def accept(logits: Optional[torch.Tensor], draft: torch.Tensor, parent: torch.Te
     ws = torch.empty(max(int(need.value), 16), dtype=torch.uint8, device=dev)
     a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
     _lib.check(lib.tv_accept(ctypes.byref(a), _lib.stream_ptr(dev)), "tv_accept")
+    return AcceptResult(nxt, res, m)
+
+
+def accept_residual(logits: torch.Tensor, draft: torch.Tensor, parent: torch.Tensor, uniform: torch.Tensor, *,
+                    draft_probs: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                    counts: Optional[torch.Tensor] = None) -> AcceptResult:
+    """Acceptance by the residual rule of speculative sampling, from given
+    uniform numbers (``tv_residual_accept``): accepted drafts and the token
+    drawn after them are distributed as samples of ``softmax(logits /
+    temperature)``, whatever the draft proposed.  :func:`accept` samples one
+    token per node and matches the drafts against it instead.
+
+    One tree: logits [M, V] (bf16, fp16 or fp32), draft [M] (the root first),
+    parent [M - 1] (-1: child of the root; a parent comes before its
+    children), uniform [M] fp32 in [0, 1): ``uniform[i]`` decides node i's
+    draft, ``uniform[0]`` draws the final token.  A batch has a leading
+    dimension everywhere; ``counts`` (int32 [B], or [1]) is then each
+    sequence's number of nodes, the rest being padding that is not read.
+
+    ``draft_probs`` None: the drafts are fixed (the draft's top-k); with
+    ``draft_probs`` [.., M, V] each node's children were drawn independently
+    from its row (rows of nodes without children are not read).
+
+    ``result`` is :func:`accept`'s ([8 + 2M], or [B, 8 + 2M]; unused path
+    entries -1) and ``next_tokens`` holds the drawn token at the last accepted
+    node and -1 elsewhere.  Invalid values in a sequence (parents, drafted
+    tokens, a row without a finite logit) are reported by ``to_host``.
+    """
+    dev = _lib.require_cuda(logits, draft, parent, uniform, draft_probs, counts)
+    single = logits.dim() == 2
+    lead = (1,) if single else tuple(logits.shape[:1])
+    if logits.dim() != (2 if single else 3) or logits.shape[-2] < 1 or logits.shape[-1] < 1:
+        raise _lib.SpecVerifyError(-1, f"logits must be [M, V] or [B, M, V], got {tuple(logits.shape)}")
+    m, v = logits.shape[-2], logits.shape[-1]
+    b = lead[0]
+    own = () if single else lead
+    for what, t, shape, dtype in (("draft", draft, own + (m,), torch.int64), ("parent", parent, own + (m - 1,), torch.int64),
+                                  ("uniform", uniform, own + (m,), torch.float32), ("counts", counts, (b,), torch.int32),
+                                  ("draft_probs", draft_probs, own + (m, v), None)):
+        if t is None:
+            continue
+        if tuple(t.shape) != shape:
+            raise _lib.SpecVerifyError(-1, f"{what} must be {list(shape)}, got {list(t.shape)}")
+        if dtype is not None and t.dtype != dtype:
+            raise _lib.SpecVerifyError(-2, f"{what} must be {dtype}, got {t.dtype}")
+        if t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise _lib.SpecVerifyError(-3, f"{what} must have unit stride on its last dimension")
+    if v > 1 and logits.stride(-1) != 1:
+        raise _lib.SpecVerifyError(-3, "logits must have unit stride on the vocabulary")
+    a = _lib.ResidualAcceptArgs()
+    a.logits_dtype, a.batch, a.rows, a.vocab = _lib.dtype_code(logits.dtype), b, m, v
+    a.logits, a.logits_sb, a.logits_sm = logits.data_ptr(), 0 if single else logits.stride(0), logits.stride(-2)
+    a.draft, a.draft_sb = draft.data_ptr(), 0 if single else draft.stride(0)
+    a.parent, a.parent_sb = parent.data_ptr(), 0 if single else parent.stride(0)
+    a.uniform, a.uniform_sb = uniform.data_ptr(), 0 if single else uniform.stride(0)
+    if counts is not None:
+        a.counts = counts.data_ptr()
+    if draft_probs is not None:
+        a.probs_dtype, a.probs = _lib.dtype_code(draft_probs.dtype), draft_probs.data_ptr()
+        a.probs_sb, a.probs_sm = 0 if single else draft_probs.stride(0), draft_probs.stride(-2)
+    a.temperature = float(temperature)
+    nxt = torch.empty(own + (m,), dtype=torch.int64, device=dev)
+    res = torch.empty(own + (RESULT_HEADER + 2 * m,), dtype=torch.int64, device=dev)
+    a.next_tokens, a.result = nxt.data_ptr(), res.data_ptr()
+    lib = _lib.load()
+    need = ctypes.c_size_t(0)
+    _lib.check(lib.tv_residual_accept_workspace_size(ctypes.byref(a), ctypes.byref(need)),
+               "tv_residual_accept_workspace_size")
+    ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), need.value
+    _lib.check(_lib.launch(dev, lib.tv_residual_accept, ctypes.byref(a)), "tv_residual_accept")
     return AcceptResult(nxt, res, m)
 
 

@@ -2,6 +2,7 @@
 
 from .bundle_verifier import FusedBundleVerifier, PagedBundleVerifier
 from .cache_state import KVCache, initialize_past_key_values
+from .lowbit import add_rms_norm
 from .rotary import apply_rotary_pos_emb, apply_rotary_pos_emb_L31, rope_append
 from .tree_attention import (KERNELS_AVAILABLE, TRITON_AVAILABLE, attention, describe_attention,
                              mask_word_summary, pack_tree_mask, prefix_attention_forward, tree_attention_forward,
@@ -12,6 +13,7 @@ __all__ = [
     "PagedBundleVerifier",
     "KVCache",
     "initialize_past_key_values",
+    "add_rms_norm",
     "apply_rotary_pos_emb",
     "apply_rotary_pos_emb_L31",
     "rope_append",

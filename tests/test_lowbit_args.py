@@ -1,0 +1,76 @@
+"""Argument checks of the low-bit and residual-rule entries, host only (the
+pointers are never used: every refusal comes before a launch)."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from specverify import SpecVerifyError, _lib
+
+FAKE = 1 << 20
+
+
+@pytest.fixture(scope="module")
+def lib():
+    import build
+    build.build()
+    return _lib.load()
+
+
+def test_add_rms_norm_checks(lib):
+    f = lib.tv_add_rms_norm
+    good = dict(x=FAKE, xs=64, r=FAKE, rs=64, w=FAKE, h=FAKE, hs=64, y=FAKE, ys=64, s=None, rows=4, cols=64, eps=1e-5,
+                dt=0)
+
+    def call(**kw):
+        return f(*{**good, **kw}.values(), None)
+    assert call(rows=0) == 0                     # nothing to do
+    assert call(rows=-1) == -1 and call(cols=0) == -1
+    assert call(dt=2) == -2 and call(dt=7) == -2
+    for k in "xrwhy":
+        assert call(**{k: None}) == -8, k
+
+
+def _accept(**kw):
+    a = _lib.ResidualAcceptArgs()
+    a.logits_dtype, a.batch, a.rows, a.vocab = 0, 2, 3, 100
+    a.logits = a.draft = a.parent = a.uniform = a.next_tokens = a.result = FAKE
+    a.temperature = 1.0
+    a.workspace, a.workspace_bytes = FAKE, 1 << 16
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+def test_residual_accept_checks(lib):
+    def call(**kw):
+        return lib.tv_residual_accept(ctypes.byref(_accept(**kw)), None)
+    assert call(batch=0) == 0
+    assert call(batch=-1) == -1 and call(rows=0) == -1 and call(vocab=0) == -1
+    assert call(rows=1025) == -7 and call(batch=65536) == -7 and call(vocab=(1 << 30) + 1) == -7
+    assert call(logits_dtype=3) == -2 and call(probs=FAKE, probs_dtype=-1) == -2
+    for t in (0.0, -1.0, float("nan"), float("inf")):
+        assert call(temperature=t) == -6, t
+    for k in ("logits", "draft", "parent", "uniform", "next_tokens", "result"):
+        assert call(**{k: None}) == -8, k
+    assert call(workspace=None) == -5 and call(workspace_bytes=8) == -5
+    assert call(workspace=FAKE + 8) == -3
+    assert lib.tv_residual_accept(None, None) == -8
+    n = ctypes.c_size_t(0)
+    assert lib.tv_residual_accept_workspace_size(ctypes.byref(_accept(rows=65, vocab=128256)), ctypes.byref(n)) == 0
+    assert n.value == 2 * 65 * 16 * 12 + 16      # 8192 16-bit words a chunk: 16 (max, sum) pairs a row
+    assert lib.tv_residual_accept_workspace_size(ctypes.byref(_accept()), None) == -8
+
+
+def test_cpu_tensors_are_refused():
+    from specverify.draft import accept_residual
+    from specverify.runtime import add_rms_norm
+    x = torch.zeros(2, 8, dtype=torch.bfloat16)
+    with pytest.raises(SpecVerifyError):
+        add_rms_norm(x, x, x[0], 1e-5)
+    with pytest.raises(SpecVerifyError):
+        accept_residual(torch.zeros(2, 8), torch.zeros(2, dtype=torch.int64), torch.zeros(1, dtype=torch.int64),
+                        torch.zeros(2))
