@@ -44,6 +44,8 @@
  *   tv_gather_rows        diffspec/draft/draft_network.py:1514-1612 (retrieval)
  *   tv_residual_accept    no counterpart (diffspec/draft/tree_verification.py:100-162
  *                         samples and matches)
+ *   tv_w4_linear          the nn.Linear projections of diffspec/runtime/
+ *                         llama_target_model.py:506-538, :765-783 in 4 bits
  *   tv_add_rms_norm       diffspec/runtime/llama_target_model.py:124-138 (LlamaRMSNorm)
  *                         with the residual's addition before it
  */
@@ -70,7 +72,7 @@ enum tv_status {
   TV_ERR_NULL = -8         /* required pointer is NULL                    */
 };
 
-enum tv_dtype { TV_BF16 = 0, TV_F16 = 1, TV_F32 = 2 };
+enum tv_dtype { TV_BF16 = 0, TV_F16 = 1, TV_F32 = 2, TV_E4M3 = 3 /* tv_w4_linear's x only */ };
 
 /* Human-readable text for a status code (static storage). */
 const char* tv_status_string(int status);
@@ -586,6 +588,37 @@ int tv_add_rms_norm(const void* x, int64_t x_row_stride, const void* residual, i
                     const void* weight, void* residual_out, int64_t residual_out_row_stride, void* y,
                     int64_t y_row_stride, float* y_scale, int32_t rows, int32_t cols, float eps, int32_t dtype,
                     void* stream);
+
+/* ---- 4-bit weights ---------------------------------------------------------------
+ * Rows times 4-bit weights with group scales (the reference's nn.Linear
+ * projections, runtime/llama_target_model.py:506-538 and :765-783, with their
+ * weights in 4 bits), for every row t < rows and output n:
+ *   out[t, n] = x_scale[t] * sum_k x[t, k] * (u[n, k] - 8) * scales[n, k / group]
+ * u: unsigned nibbles, eight per 32-bit word: word c of row n holds
+ *   k = 8 c + {0, 2, 4, 6, 1, 3, 5, 7} from the lowest nibble up
+ *   (q_sn words between rows, a multiple of 4; 16-byte aligned).
+ * scales [n][k / group], row stride s_sn; group a multiple of 32, k a multiple
+ * of group.  x [rows][k] (row stride x_sm): out_dtype (bf16 or fp16, also the
+ * scales' type), or TV_E4M3 with x_scale [rows] fp32 (NULL otherwise).
+ * out [rows][n], row stride o_sm.  Sums are in fp32.  rows == 0 does nothing. */
+typedef struct tv_w4_args {
+  int32_t x_dtype, out_dtype;
+  int32_t rows, n, k, group;
+  const void* x;
+  int64_t x_sm;
+  const float* x_scale;
+  const void* qweight;
+  int64_t q_sn;
+  const void* scales;
+  int64_t s_sn;
+  void* out;
+  int64_t o_sm;
+  void* workspace;
+  size_t workspace_bytes;
+} tv_w4_args;
+
+int tv_w4_workspace_size(const tv_w4_args* args, size_t* bytes);
+int tv_w4_linear(const tv_w4_args* args, void* stream);
 
 #ifdef __cplusplus
 }

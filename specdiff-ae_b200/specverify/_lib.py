@@ -16,7 +16,7 @@ import torch
 LIB_PATH = Path(__file__).resolve().parent / "libspecverify.so"
 
 TV_OK = 0
-TV_BF16, TV_F16, TV_F32 = 0, 1, 2
+TV_BF16, TV_F16, TV_F32, TV_E4M3 = 0, 1, 2, 3
 
 _DTYPE_CODE = {torch.bfloat16: TV_BF16, torch.float16: TV_F16, torch.float32: TV_F32}
 
@@ -111,6 +111,16 @@ class ResidualAcceptArgs(ctypes.Structure):
     ]
 
 
+class W4Args(ctypes.Structure):
+    """Mirror of ``tv_w4_args``."""
+    _fields_ = [
+        ("x_dtype", c_i32), ("out_dtype", c_i32), ("rows", c_i32), ("n", c_i32), ("k", c_i32), ("group", c_i32),
+        ("x", c_vp), ("x_sm", c_i64), ("x_scale", c_vp), ("qweight", c_vp), ("q_sn", c_i64),
+        ("scales", c_vp), ("s_sn", c_i64), ("out", c_vp), ("o_sm", c_i64),
+        ("workspace", c_vp), ("workspace_bytes", c_size),
+    ]
+
+
 # name -> (restype, argtypes)
 _SIGNATURES = {
     "tv_status_string": (ctypes.c_char_p, [c_i32]),
@@ -149,6 +159,8 @@ _SIGNATURES = {
     "tv_rms_norm": (c_i32, [c_vp, c_i64, c_vp, c_vp, c_i64, c_i32, c_i32, c_f32, c_i32, c_vp]),
     "tv_add_rms_norm": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_i32, c_i32, c_f32,
                                 c_i32, c_vp]),
+    "tv_w4_workspace_size": (c_i32, [ctypes.POINTER(W4Args), ctypes.POINTER(c_size)]),
+    "tv_w4_linear": (c_i32, [ctypes.POINTER(W4Args), c_vp]),
     "tv_silu_mul": (c_i32, [c_vp, c_vp, c_i64, c_vp, c_i64, c_i32, c_i32, c_i32, c_vp]),
 }
 

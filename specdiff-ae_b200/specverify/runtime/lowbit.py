@@ -9,13 +9,14 @@ CUDA tensors only; errors raise :class:`specverify.SpecVerifyError`.
 
 from __future__ import annotations
 
+import ctypes
 from typing import Optional, Tuple, Union
 
 import torch
 
 from .. import _lib
 
-__all__ = ["add_rms_norm"]
+__all__ = ["add_rms_norm", "dequantize_w4", "quantize_w4", "w4_linear"]
 
 _HALF = (torch.bfloat16, torch.float16)
 
@@ -66,3 +67,100 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, 
                      _lib.TV_BF16 if x.dtype == torch.bfloat16 else _lib.TV_F16)
     _lib.check(st, "tv_add_rms_norm")
     return (y, scale, residual_out) if fp8 else (y, residual_out)
+
+
+# nibble i of a packed word holds weight 8 c + _ORDER[i]
+_ORDER = (0, 2, 4, 6, 1, 3, 5, 7)
+
+
+def quantize_w4(weight: torch.Tensor, group: int = 128) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Round a weight [N, K] (bf16 or fp16) to 4 bits with a scale per ``group``
+    consecutive k of a row: ``scale = max|w| / 7`` rounded to the weight's type,
+    ``q = round(w / scale)`` in -8 .. 7.  Returns ``(qweight, scales)``: int32
+    [N, K / 8] (layout at ``tv_w4_linear``) and [N, K / group].  Plain torch
+    operations on the weight's device, done once when a model is loaded.
+    """
+    if weight.dim() != 2 or weight.dtype not in _HALF:
+        raise _lib.SpecVerifyError(-1, f"weight must be [N, K] in bfloat16 or float16, got {tuple(weight.shape)} "
+                                       f"{weight.dtype}")
+    n, k = weight.shape
+    if group < 32 or group % 32 or k < group or k % group:
+        raise _lib.SpecVerifyError(-1, f"group {group} must be a multiple of 32 that divides K {k}")
+    w = weight.float().view(n, k // group, group)
+    scales = (w.abs().amax(-1) / 7.0).to(weight.dtype)
+    s = scales.float()[:, :, None]
+    u = torch.where(s > 0, torch.round(w / s), 0.0).clamp(-8, 7).to(torch.int32).view(n, k // 8, 8) + 8
+    q = torch.zeros((n, k // 8), dtype=torch.int32, device=weight.device)
+    for i, o in enumerate(_ORDER):
+        q |= u[:, :, o] << (4 * i)
+    return q, scales
+
+
+def dequantize_w4(qweight: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """The weight [N, K] that ``(qweight, scales)`` stand for, in the scales' type."""
+    n, k = qweight.shape[0], qweight.shape[1] * 8
+    u = torch.empty((n, k // 8, 8), dtype=torch.float32, device=qweight.device)
+    for i, o in enumerate(_ORDER):
+        u[:, :, o] = ((qweight >> (4 * i)) & 15).float() - 8.0
+    w = u.view(n, scales.shape[1], -1) * scales.float()[:, :, None]
+    return w.view(n, k).to(scales.dtype)
+
+
+def w4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, *, x_scale: Optional[torch.Tensor] = None,
+              out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x @ W.T`` for a 4-bit weight W [N, K] (``tv_w4_linear``).
+
+    x [..., K]: the scales' type (bf16 or fp16), or float8_e4m3fn with
+    ``x_scale`` (fp32, one per row, shape [...]) as :func:`add_rms_norm`
+    returns them; unit stride on K.  qweight [N, K / 8] int32 and scales
+    [N, K / group] as :func:`quantize_w4` lays them out (group a multiple of
+    32).  Returns [..., N] in the scales' type, summed in fp32; ``out``, when
+    given, is [rows, N] with unit stride on N.
+    """
+    dev = _lib.require_cuda(x, qweight, scales, x_scale, out)
+    if x.dim() < 1 or qweight.dim() != 2 or scales.dim() != 2 or qweight.shape[0] != scales.shape[0]:
+        raise _lib.SpecVerifyError(-1, f"x {tuple(x.shape)}, qweight {tuple(qweight.shape)}, scales "
+                                       f"{tuple(scales.shape)}")
+    n, k = qweight.shape[0], qweight.shape[1] * 8
+    groups = scales.shape[1]
+    if x.shape[-1] != k or groups < 1 or k % groups or (k // groups) % 32 or n < 1:
+        raise _lib.SpecVerifyError(-1, f"x {tuple(x.shape)} and scales {tuple(scales.shape)} do not fit a "
+                                       f"[{n}, {k}] weight with groups of a multiple of 32")
+    if qweight.dtype != torch.int32 or scales.dtype not in _HALF:
+        raise _lib.SpecVerifyError(-2, f"qweight {qweight.dtype} must be int32, scales {scales.dtype} 16-bit")
+    fp8 = x.dtype == torch.float8_e4m3fn
+    if not fp8 and x.dtype != scales.dtype:
+        raise _lib.SpecVerifyError(-2, f"x {x.dtype} must be {scales.dtype} or float8_e4m3fn")
+    if fp8 != (x_scale is not None):
+        raise _lib.SpecVerifyError(-8, "x_scale goes with a float8_e4m3fn x, and only with it")
+    x2 = x if x.dim() == 2 else x.reshape(-1, k)
+    rows = x2.shape[0]
+    if x2.stride(1) != 1 or qweight.stride(1) != 1 or (groups > 1 and scales.stride(1) != 1):
+        raise _lib.SpecVerifyError(-3, "x, qweight and scales must have unit stride on their last dimension")
+    if fp8 and (x_scale.dtype != torch.float32 or x_scale.shape != x.shape[:-1] or not x_scale.is_contiguous()):
+        raise _lib.SpecVerifyError(-1, f"x_scale must be a contiguous float32 {list(x.shape[:-1])}")
+    if out is None:
+        res = torch.empty(x.shape[:-1] + (n,), dtype=scales.dtype, device=dev)
+        o_sm = n
+    else:
+        if out.shape != (rows, n) or out.dtype != scales.dtype or (n > 1 and out.stride(1) != 1) or (
+                rows > 1 and out.stride(0) < n):
+            raise _lib.SpecVerifyError(-1, f"out must be [{rows}, {n}] {scales.dtype} with unit column stride")
+        res, o_sm = out, out.stride(0)
+    a = _lib.W4Args()
+    a.out_dtype = _lib.TV_BF16 if scales.dtype == torch.bfloat16 else _lib.TV_F16
+    a.x_dtype = _lib.TV_E4M3 if fp8 else a.out_dtype
+    a.rows, a.n, a.k, a.group = rows, n, k, k // groups
+    a.x, a.x_sm = x2.data_ptr(), x2.stride(0)
+    a.x_scale = x_scale.data_ptr() if fp8 else None
+    a.qweight, a.q_sn = qweight.data_ptr(), qweight.stride(0)
+    a.scales, a.s_sn = scales.data_ptr(), scales.stride(0)
+    a.out, a.o_sm = res.data_ptr(), o_sm
+    lib = _lib.load()
+    need = ctypes.c_size_t(0)
+    _lib.check(lib.tv_w4_workspace_size(ctypes.byref(a), ctypes.byref(need)), "tv_w4_workspace_size")
+    if need.value:
+        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need.value
+    _lib.check(_lib.launch(dev, lib.tv_w4_linear, ctypes.byref(a)), "tv_w4_linear")
+    return res

@@ -74,3 +74,30 @@ def test_cpu_tensors_are_refused():
     with pytest.raises(SpecVerifyError):
         accept_residual(torch.zeros(2, 8), torch.zeros(2, dtype=torch.int64), torch.zeros(1, dtype=torch.int64),
                         torch.zeros(2))
+
+
+def test_w4_linear_checks(lib):
+    def args(**kw):
+        a = _lib.W4Args()
+        a.x_dtype = a.out_dtype = 0
+        a.rows, a.n, a.k, a.group = 4, 100, 256, 64
+        a.x = a.qweight = a.scales = a.out = FAKE
+        a.x_sm, a.q_sn, a.s_sn, a.o_sm = 256, 32, 4, 100
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return a
+
+    def call(**kw):
+        return lib.tv_w4_linear(ctypes.byref(args(**kw)), None)
+    assert call(rows=0) == 0
+    assert call(rows=-1) == -1 and call(n=0) == -1 and call(k=0) == -1
+    assert call(group=48) == -1 and call(group=0) == -1 and call(group=96) == -1 and call(group=512) == -1
+    assert call(out_dtype=2) == -2 and call(x_dtype=1) == -2 and call(x_dtype=2) == -2
+    for k in ("x", "qweight", "scales", "out"):
+        assert call(**{k: None}) == -8, k
+    assert call(x_dtype=3) == -8                                # e4m3 rows need their scales
+    assert call(qweight=FAKE + 4) == -3 and call(q_sn=33) == -3
+    assert lib.tv_w4_linear(None, None) == -8
+    n = ctypes.c_size_t(0)
+    assert lib.tv_w4_workspace_size(ctypes.byref(args()), ctypes.byref(n)) == 0
+    assert lib.tv_w4_workspace_size(None, ctypes.byref(n)) == -8
