@@ -1,73 +1,505 @@
-// Rows times 4-bit weights with group scales:
+// Rows times 4-bit weights with group scales (sm_100a):
 //
 //   y[t, n] = xs[t] * sum_k x[t, k] * (u[n, k] - 8) * s[n, k / group]
 //
-// One warp per weight row and block of tokens: a lane takes every 32nd word of
-// eight weights, sums its products in fp32 and scales each word's sum.
+// A CTA takes 128 weight rows (the M of tcgen05.mma, one TMEM lane each), up
+// to 128 tokens (its N) and a range of k.  The packed weights stream through a
+// shared-memory ring (TMA, 128 rows x 128 k = 8 KB a stage).  Eight warps, two
+// groups of four, turn them into 16-bit values, a thread its own weight row,
+// and write those straight into tensor memory, where the MMA reads its A
+// operand; x comes by TMA as the B operand in 64-k tiles.
+//
+//   warp 0      weight producer (TMA)
+//   warp 1      MMA issuer, tensor-memory owner
+//   warp 2      x producer (TMA)
+//   warps 4-11  weights to 16 bits (group w / 4 - 1 takes every other stage),
+//               then the epilogue (TMEM lane quarter w mod 4)
+//
+// Where there are fewer tiles than CTAs that fit the GPU, a cluster of up to 8
+// CTAs splits k; the partial sums meet in distributed shared memory and are
+// added in rank order, so results do not depend on timing.
+//
+// Bound by HBM (the packed weights once) up to about 80 tokens, by the tensor
+// pipe above.  Each (u - 8) * s is rounded once to x's 16-bit type (the MMA
+// takes no other): half a step, as the weight itself had in that type.
+#include <cooperative_groups.h>
+#include <cuda.h>
 #include <cuda_fp8.h>
+#include <cudaTypedefs.h>
+
+#include <mutex>
+#include <type_traits>
 
 #include "common.cuh"
+#include "sm100.cuh"
 
 namespace tv {
 namespace {
 
-constexpr int kTokens = 4;       // tokens per warp
+using namespace sm100;
+namespace cg = cooperative_groups;
+
+constexpr int kRows = 128;                   // weight rows per CTA
+constexpr int kMaxTokens = 128;              // tokens per CTA
+constexpr int kStageK = 128;                 // k per weight stage
+constexpr int kWStage = kRows * kStageK / 2; // 8 KB
+constexpr int kThreads = 384;
+constexpr int kDequantWarp = 4;              // first of the eight
+constexpr int kMaxStages = 12;
+constexpr int kRing = 112 * 1024;            // both rings: two CTAs share an SM
+constexpr int kSmem = kRing + 1024;
+constexpr uint32_t kTmemCols = 256;          // two CTAs per SM
+constexpr uint32_t kACol = 128;              // accumulator in columns 0-127, four 32-column A buffers after it
+constexpr int kMaxCluster = 8;
+constexpr int kSlots = 2 * kNumSMs;
+
+struct Bars {
+  uint64_t w_full[kMaxStages], w_empty[kMaxStages];
+  uint64_t x_full[kMaxStages], x_empty[kMaxStages];
+  uint64_t a_full[4], a_empty[4];
+  uint64_t done;
+  uint32_t tmem;
+  int abort;
+};
+static_assert(sizeof(Bars) <= kSmem - kRing, "barrier block");
 
 struct W4Params {
-  const void* x;
-  int64_t x_sm;
-  const float* x_scale;
-  const uint32_t* q;
-  int64_t q_sn;
   const void* s;
   int64_t s_sn;
+  const float* x_scale;
   void* out;
   int64_t o_sm;
-  int rows, n, k, group;
+  int rows, n, k;
+  int tokens;                  // N of the MMA: tokens per CTA, a multiple of 16
+  int w_stages, x_stages, x_bytes;
+  int split;                   // CTAs of a cluster
+  uint32_t group_magic;        // k / group = (k / 32) * magic >> 32; 0: group 32
 };
 
-template <typename X> __device__ __forceinline__ float x_float(X v) { return Elem<X>::to_f(v); }
-template <> __device__ __forceinline__ float x_float<__nv_fp8_e4m3>(__nv_fp8_e4m3 v) { return static_cast<float>(v); }
+template <typename T> __device__ __forceinline__ T bits_as(uint32_t u) { return *reinterpret_cast<T*>(&u); }
+template <typename T> __device__ __forceinline__ uint32_t as_bits(T v) { return *reinterpret_cast<uint32_t*>(&v); }
 
-template <typename X, typename T>
-__global__ void __launch_bounds__(256) w4_kernel(const W4Params a) {
-  const int lane = threadIdx.x & 31;
-  const int n = blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int t0 = blockIdx.y * kTokens;
-  if (n >= a.n) return;
-  const uint32_t* q = a.q + (int64_t)n * a.q_sn;
-  const T* s = static_cast<const T*>(a.s) + (int64_t)n * a.s_sn;
-  float acc[kTokens] = {};
-  for (int c = lane; c < a.k / 8; c += 32) {
-    const uint32_t w = q[c];
-    const float sc = Elem<T>::to_f(s[c * 8 / a.group]);
-#pragma unroll
-    for (int i = 0; i < kTokens; ++i) {
-      if (t0 + i >= a.rows) break;
-      const X* x = static_cast<const X*>(a.x) + (int64_t)(t0 + i) * a.x_sm + c * 8;
-      float d = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        d = fmaf(x_float<X>(x[2 * j]), (float)((int)((w >> (4 * j)) & 15) - 8), d);
-        d = fmaf(x_float<X>(x[2 * j + 1]), (float)((int)((w >> (4 * j + 16)) & 15) - 8), d);
+// Eight packed weights -> four pairs of 16-bit values in k order.
+//
+// bf16: the bits 0 .. 255 read as a bf16 are that integer times 2^-133 (the
+// subnormal range and the first binade share a spacing), so a nibble masked at
+// bits 0-3 is u * 2^-133 and one at bits 4-7 is u * 2^-129, and ONE fused
+// multiply-add, (u * 2^-133) * (s * 2^(133 - 40)) - 8 s * 2^-40, gives
+// (u - 8) * s * 2^-40 rounded once: both factors and the addend are exact.
+// The accumulator is multiplied by 2^40 at the end.  Scales from 2^-80 to
+// 2^30 stay inside the exponent range.  9 instructions for 8 weights; the
+// usual 128 + u form needs a subtraction and a product, 15.
+//
+// fp16's exponents are too few for that: 1024 + u (or 1024 + 16 u), made by
+// OR, loses its offset in one exact operation, then the product rounds once.
+template <typename T> struct Unpack;
+template <> struct Unpack<__nv_bfloat16> {
+  __nv_bfloat162 sa, sb, off;
+  __device__ __forceinline__ void scale(__nv_bfloat16 s) {
+    const float f = __bfloat162float(s);
+    sa = __float2bfloat162_rn(f * 9.903520314283042e27f);      // 2^93
+    sb = __float2bfloat162_rn(f * 6.189700196426902e26f);      // 2^89
+    off = __float2bfloat162_rn(f * -7.275957614183426e-12f);   // -2^-37
+  }
+  __device__ __forceinline__ void word(uint32_t w, uint32_t* o) const {
+    const uint32_t v = w >> 8;
+    o[0] = as_bits(__hfma2(bits_as<__nv_bfloat162>(w & 0x000F000Fu), sa, off));
+    o[1] = as_bits(__hfma2(bits_as<__nv_bfloat162>(w & 0x00F000F0u), sb, off));
+    o[2] = as_bits(__hfma2(bits_as<__nv_bfloat162>(v & 0x000F000Fu), sa, off));
+    o[3] = as_bits(__hfma2(bits_as<__nv_bfloat162>(v & 0x00F000F0u), sb, off));
+  }
+  static __device__ __forceinline__ float unscale() { return 1099511627776.0f; }   // 2^40
+};
+template <> struct Unpack<__half> {
+  __half2 s2;
+  __device__ __forceinline__ void scale(__half s) { s2 = __half2half2(s); }
+  __device__ __forceinline__ void word(uint32_t w, uint32_t* o) const {
+    const uint32_t v = w >> 8;
+    const __half2 lo = __float2half2_rn(-1032.f), sixteenth = __float2half2_rn(0.0625f), hi = __float2half2_rn(-72.f);
+    o[0] = as_bits(__hmul2(__hadd2(bits_as<__half2>((w & 0x000F000Fu) | 0x64006400u), lo), s2));
+    o[1] = as_bits(__hmul2(__hfma2(bits_as<__half2>((w & 0x00F000F0u) | 0x64006400u), sixteenth, hi), s2));
+    o[2] = as_bits(__hmul2(__hadd2(bits_as<__half2>((v & 0x000F000Fu) | 0x64006400u), lo), s2));
+    o[3] = as_bits(__hmul2(__hfma2(bits_as<__half2>((v & 0x00F000F0u) | 0x64006400u), sixteenth, hi), s2));
+  }
+  static __device__ __forceinline__ float unscale() { return 1.0f; }
+};
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr));
+}
+
+// Loads in flight land before shared memory is reused or released: a producer
+// ends by waiting for its last loads whatever the abort flag says, 0.2 s each.
+__device__ __forceinline__ void drain(uint64_t* full, int stages, int it) {
+  volatile int keep_waiting = 0;
+  for (int j = it > stages ? it - stages : 0; j < it; ++j)
+    mbar_wait(&full[j % stages], (j / stages) & 1, &keep_waiting, 200000000ull);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2)
+    w4_kernel(const __grid_constant__ CUtensorMap tmw, const __grid_constant__ CUtensorMap tmx, const W4Params p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  Bars* bars = reinterpret_cast<Bars*>(smem + kRing);
+  volatile int* abort = &bars->abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = blockIdx.x % p.split;
+  const int n0 = blockIdx.x / p.split * kRows;
+  const int t0 = blockIdx.y * p.tokens;
+  // this CTA's weight stages
+  const int all = (p.k + kStageK - 1) / kStageK;
+  const int kb0 = (int)((int64_t)all * rank / p.split);
+  const int nb = (int)((int64_t)all * (rank + 1) / p.split) - kb0;
+  uint8_t* w_ring = smem;
+  uint8_t* x_ring = smem + p.w_stages * kWStage;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < p.w_stages; ++i) {
+      mbar_init(&bars->w_full[i], 1);
+      mbar_init(&bars->w_empty[i], 4);
+    }
+    for (int i = 0; i < p.x_stages; ++i) {
+      mbar_init(&bars->x_full[i], 1);
+      mbar_init(&bars->x_empty[i], 1);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&bars->a_full[i], 4);
+      mbar_init(&bars->a_empty[i], 1);
+    }
+    mbar_init(&bars->done, 1);
+    bars->abort = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&bars->tmem, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int s = 0, ph = 1, i = 0;
+      bool ok = true;
+      for (; i < nb; ++i) {
+        if (i >= p.w_stages && !mbar_wait(&bars->w_empty[s], ph, abort)) {
+          ok = false;
+          break;
+        }
+        mbar_arrive_expect_tx(&bars->w_full[s], kWStage);
+        tma_load_2d(w_ring + s * kWStage, &tmw, &bars->w_full[s], (kb0 + i) * (kStageK / 2), n0);
+        if (++s == p.w_stages) {
+          s = 0;
+          ph ^= 1;
+        }
       }
-      acc[i] = fmaf(d, sc, acc[i]);
+      if (!ok) bars->abort = 1;
+      drain(bars->w_full, p.w_stages, i);
+    }
+  } else if (warp == 2) {
+    if (lane == 0) {
+      int s = 0, ph = 1, i = 0;
+      bool ok = true;
+      for (; i < 2 * nb; ++i) {
+        if (i >= p.x_stages && !mbar_wait(&bars->x_empty[s], ph, abort)) {
+          ok = false;
+          break;
+        }
+        mbar_arrive_expect_tx(&bars->x_full[s], p.x_bytes);
+        tma_load_2d(x_ring + s * p.x_bytes, &tmx, &bars->x_full[s], (2 * kb0 + i) * 64, t0);
+        if (++s == p.x_stages) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+      if (!ok) bars->abort = 1;
+      drain(bars->x_full, p.x_stages, i);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+      const uint32_t idesc = idesc_f16(fmt, kRows, (uint32_t)p.tokens, 0);
+      int xs = 0, xph = 0;
+      bool ok = true;
+      for (int i = 0; ok && i < nb; ++i) {
+        for (int h = 0; h < 2; ++h) {
+          const int buf = (i & 1) * 2 + h;
+          if (!mbar_wait(&bars->x_full[xs], xph, abort) || !mbar_wait(&bars->a_full[buf], (i >> 1) & 1, abort)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t b = smem_u32(x_ring + xs * p.x_bytes);
+          const uint32_t a = tmem + kACol + (uint32_t)(buf * 32);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_ts(tmem, a + kk * 8, smem_desc_sw128(b + kk * 32, 16, 1024), idesc, (i | h | kk) ? 1u : 0u);
+          tc_commit(&bars->a_empty[buf]);
+          tc_commit(&bars->x_empty[xs]);
+          if (++xs == p.x_stages) {
+            xs = 0;
+            xph ^= 1;
+          }
+        }
+      }
+      if (ok) tc_commit(&bars->done);
+      else bars->abort = 1;
+    }
+  } else if (warp >= kDequantWarp) {
+    const int g = (warp - kDequantWarp) >> 2;
+    const int q4 = warp & 3;
+    const int r = q4 * 32 + lane;                        // weight row = TMEM lane
+    const uint32_t lanes = tmem + ((uint32_t)(q4 * 32) << 16);
+    const T* srow = static_cast<const T*>(p.s) + (int64_t)min(n0 + r, p.n - 1) * p.s_sn;
+    const int units = n0 + r < p.n ? p.k / 32 : 0;       // 32-k units of this row; scale 0 past the end
+    auto scale_at = [&](int u) {
+      if (u >= units) return Elem<T>::from_f(0.f);
+      return srow[p.group_magic ? __umulhi((uint32_t)u, p.group_magic) : (uint32_t)u];
+    };
+    T sc[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) sc[b] = scale_at((kb0 + g) * 4 + b);
+    int s = g, ph = 0;
+    bool ok = true;
+    for (int i = g; i < nb; i += 2) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&bars->w_full[s], ph, abort))) {
+        ok = false;
+        break;
+      }
+      uint4 w[4];
+      const uint8_t* src = w_ring + s * kWStage + r * 64;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) w[c] = *reinterpret_cast<const uint4*>(src + ((c ^ ((r >> 1) & 3)) << 4));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->w_empty[s]);
+      Unpack<T> un[4];
+#pragma unroll
+      for (int b = 0; b < 4; ++b) un[b].scale(sc[b]);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) sc[b] = scale_at((kb0 + i + 2) * 4 + b);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t o[32];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const Unpack<T>& u = un[h * 2 + c];
+          const uint4 v = w[h * 2 + c];
+          u.word(v.x, o + c * 16);
+          u.word(v.y, o + c * 16 + 4);
+          u.word(v.z, o + c * 16 + 8);
+          u.word(v.w, o + c * 16 + 12);
+        }
+        const int buf = g * 2 + h;
+        // the MMAs that read this buffer's previous contents have finished
+        if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait(&bars->a_empty[buf], ((i >> 1) & 1) ^ 1, abort))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        tmem_st32(lanes + kACol + (uint32_t)(buf * 32), o);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->a_full[buf]);
+      }
+      if (!ok) break;
+      s += 2;
+      if (s >= p.w_stages) {
+        s -= p.w_stages;
+        ph ^= 1;
+      }
+    }
+    if (!ok) bars->abort = 1;
+    // ---- epilogue
+    ok = __all_sync(0xffffffffu, mbar_wait(&bars->done, 0, abort)) && ok;
+    if (!ok) bars->abort = 1;
+    tc_fence_after();
+    T* out = static_cast<T*>(p.out);
+    float* part = reinterpret_cast<float*>(smem);        // [token][weight row], once both rings are drained
+#pragma unroll 1
+    for (int c = g; c * 16 < p.tokens; c += 2) {
+      uint32_t v[16];
+      tmem_ld16(lanes + (uint32_t)(c * 16), v);
+      tmem_wait_ld();
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int t = t0 + c * 16 + j;
+        float f = __uint_as_float(v[j]) * Unpack<T>::unscale();
+        if (!ok) f = __int_as_float(0x7fc00000);
+        if (p.split > 1) part[(c * 16 + j) * kRows + r] = f;
+        else if (t < p.rows && n0 + r < p.n)
+          out[(int64_t)t * p.o_sm + n0 + r] = Elem<T>::from_f(p.x_scale ? f * p.x_scale[t] : f);
+      }
     }
   }
-#pragma unroll
-  for (int i = 0; i < kTokens; ++i) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
-    if (lane == 0 && t0 + i < a.rows)
-      static_cast<T*>(a.out)[(int64_t)(t0 + i) * a.o_sm + n] =
-          Elem<T>::from_f(acc[i] * (a.x_scale ? a.x_scale[t0 + i] : 1.f));
+  __syncwarp();
+  if (p.split > 1) {
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    if (warp >= kDequantWarp) {
+      int gave_up = 0;
+      for (int k = 0; k < p.split; ++k) gave_up |= *cluster.map_shared_rank(&bars->abort, k);
+      const int tid = threadIdx.x - kDequantWarp * 32;
+      const int r = tid & (kRows - 1);
+      float* part = reinterpret_cast<float*>(smem);
+      T* out = static_cast<T*>(p.out);
+      for (int j = rank + p.split * (tid / kRows); j < p.tokens; j += 2 * p.split) {
+        const int t = t0 + j;
+        if (t >= p.rows || n0 + r >= p.n) continue;
+        float f = 0.f;
+        for (int k = 0; k < p.split; ++k) f += *cluster.map_shared_rank(part + j * kRows + r, k);
+        if (gave_up) f = __int_as_float(0x7fc00000);
+        out[(int64_t)t * p.o_sm + n0 + r] = Elem<T>::from_f(p.x_scale ? f * p.x_scale[t] : f);
+      }
+    }
+    cluster.sync();     // no CTA leaves while another still reads its sums
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
   }
 }
 
+// x that TMA cannot read (8 bits, or rows off the 16-byte grid) -> dense 16-bit
+// rows.  Both types hold every e4m3 value exactly.
 template <typename X, typename T>
-int launch_w4(const W4Params& p, cudaStream_t st) {
-  w4_kernel<X, T><<<dim3((p.n + 7) / 8, (p.rows + kTokens - 1) / kTokens), 256, 0, st>>>(p);
-  return check_launch();
+__global__ void __launch_bounds__(256) w4_stage_kernel(const X* x, int64_t x_sm, T* y, int rows, int k) {
+  const int chunks = k / 8;
+  const int64_t total = (int64_t)rows * chunks;
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
+    const int64_t r = e / chunks;
+    const int c = (int)(e - r * chunks) * 8;
+    const X* src = x + r * x_sm + c;
+    float f[8];
+    if (sizeof(X) == 1 && (reinterpret_cast<uintptr_t>(src) & 7) == 0) {
+      const uint2 raw = *reinterpret_cast<const uint2*>(src);
+      const X* b = reinterpret_cast<const X*>(&raw);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = static_cast<float>(b[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = static_cast<float>(src[i]);
+    }
+    uint4 o;
+    uint32_t* w = reinterpret_cast<uint32_t*>(&o);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = Elem<T>::pack2(f[2 * i], f[2 * i + 1]);
+    *reinterpret_cast<uint4*>(y + r * k + c) = o;
+  }
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  });
+  return fn;
+}
+
+bool make_map(CUtensorMap* map, CUtensorMapDataType dt, CUtensorMapSwizzle swizzle, const void* base, uint64_t inner,
+              uint64_t outer, uint64_t stride_bytes, uint32_t box_inner, uint32_t box_outer) {
+  auto enc = encoder();
+  if (!enc) return false;
+  cuuint64_t dims[2] = {inner, outer};
+  cuuint64_t strides[1] = {stride_bytes};
+  cuuint32_t box[2] = {box_inner, box_outer}, estr[2] = {1, 1};
+  return enc(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// TMA reads 16-bit rows on the 16-byte grid; one row needs no stride of its own.
+bool staged(const tv_w4_args* a) {
+  return a->x_dtype == TV_E4M3 || !aligned16(a->x) || (a->rows > 1 && (a->x_sm < a->k || a->x_sm % 8 != 0));
+}
+
+template <typename T>
+int launch_w4(const tv_w4_args* a, cudaStream_t st) {
+  const void* x = a->x;
+  int64_t x_sm = a->rows > 1 ? a->x_sm : a->k;
+  if (staged(a)) {
+    T* y = static_cast<T*>(a->workspace);
+    const int64_t chunks = (int64_t)a->rows * (a->k / 8);
+    const int blocks = (int)(chunks / 256 + 1 < 4 * kNumSMs ? chunks / 256 + 1 : 4 * kNumSMs);
+    if (a->x_dtype == TV_E4M3)
+      w4_stage_kernel<__nv_fp8_e4m3, T><<<blocks, 256, 0, st>>>(static_cast<const __nv_fp8_e4m3*>(a->x), a->x_sm, y,
+                                                                a->rows, a->k);
+    else
+      w4_stage_kernel<T, T><<<blocks, 256, 0, st>>>(static_cast<const T*>(a->x), a->x_sm, y, a->rows, a->k);
+    const int rc = check_launch();
+    if (rc != TV_OK) return rc;
+    x = y;
+    x_sm = a->k;
+  }
+  W4Params p{};
+  p.s = a->scales;
+  p.s_sn = a->s_sn;
+  p.x_scale = a->x_dtype == TV_E4M3 ? a->x_scale : nullptr;
+  p.out = a->out;
+  p.o_sm = a->o_sm;
+  p.rows = a->rows;
+  p.n = a->n;
+  p.k = a->k;
+  p.tokens = a->rows >= kMaxTokens ? kMaxTokens : (a->rows + 15) / 16 * 16;
+  p.x_bytes = p.tokens * 128;
+  // rings: enough x tiles to cover an L2 round trip, the rest to the weights
+  p.x_stages = p.tokens <= 32 ? 8 : p.tokens <= 64 ? 6 : p.tokens <= 80 ? 5 : p.tokens <= 112 ? 4 : 3;
+  p.w_stages = (kRing - p.x_stages * p.x_bytes) / kWStage;
+  if (p.w_stages > kMaxStages) p.w_stages = kMaxStages;
+  const uint32_t g32 = (uint32_t)a->group / 32;
+  p.group_magic = g32 == 1 ? 0 : (uint32_t)(((1ull << 32) + g32 - 1) / g32);
+  const int blocks_t = (a->rows + p.tokens - 1) / p.tokens;
+  const int64_t tiles = (int64_t)((a->n + kRows - 1) / kRows) * blocks_t;
+  const int stages = (a->k + kStageK - 1) / kStageK;
+  p.split = 1;
+  while (p.split < kMaxCluster && tiles * (p.split + 1) <= kSlots && stages >= 2 * (p.split + 1)) ++p.split;
+  CUtensorMap mw, mx;
+  if (!make_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_64B, a->qweight, (uint64_t)a->k / 2,
+                (uint64_t)a->n, (uint64_t)a->q_sn * 4, kStageK / 2, kRows) ||
+      !make_map(&mx,
+                std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                      : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                CU_TENSOR_MAP_SWIZZLE_128B, x, (uint64_t)a->k, (uint64_t)a->rows, (uint64_t)x_sm * 2, 64,
+                (uint32_t)p.tokens))
+    return TV_ERR_UNSUPPORTED;
+  const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(w4_kernel<T>), kSmem);
+  if (rc != TV_OK) return rc;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((a->n + kRows - 1) / kRows * p.split), (unsigned)blocks_t);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = p.split;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, w4_kernel<T>, mw, mx, p);
+  return e == cudaSuccess ? check_launch() : record_cuda_error(e);
+}
+
+int check_shape(const tv_w4_args* a) {
+  if (a->rows < 0 || a->n < 1 || a->group < 32 || a->group % 32 != 0 || a->k < a->group || a->k % a->group != 0)
+    return TV_ERR_SHAPE;
+  if (a->out_dtype != TV_BF16 && a->out_dtype != TV_F16) return TV_ERR_DTYPE;
+  if (a->x_dtype != a->out_dtype && a->x_dtype != TV_E4M3) return TV_ERR_DTYPE;
+  // the grid's token blocks, and the scale index by multiplication
+  if (a->rows > 65535 * kMaxTokens || a->k > (1 << 20) || a->n > (1 << 27)) return TV_ERR_UNSUPPORTED;
+  return TV_OK;
 }
 
 }  // namespace
@@ -79,27 +511,28 @@ extern "C" {
 
 int tv_w4_workspace_size(const tv_w4_args* a, size_t* bytes) {
   if (!a || !bytes) return TV_ERR_NULL;
-  *bytes = 0;
+  const int rc = check_shape(a);
+  if (rc != TV_OK) return rc;
+  *bytes = a->rows > 0 && staged(a) ? (size_t)a->rows * a->k * 2 : 0;
   return TV_OK;
 }
 
 int tv_w4_linear(const tv_w4_args* a, void* stream) {
   if (!a) return TV_ERR_NULL;
-  if (a->rows < 0 || a->n < 1 || a->group < 32 || a->group % 32 != 0 || a->k < a->group || a->k % a->group != 0)
-    return TV_ERR_SHAPE;
-  if (a->out_dtype != TV_BF16 && a->out_dtype != TV_F16) return TV_ERR_DTYPE;
-  if (a->x_dtype != a->out_dtype && a->x_dtype != TV_E4M3) return TV_ERR_DTYPE;
+  const int rc = check_shape(a);
+  if (rc != TV_OK) return rc;
   if (a->rows == 0) return TV_OK;
   if (!a->x || !a->qweight || !a->scales || !a->out || (a->x_dtype == TV_E4M3 && !a->x_scale)) return TV_ERR_NULL;
   if (!aligned16(a->qweight) || a->q_sn % 4 != 0) return TV_ERR_ALIGN;
-  if (a->rows > 65535 * kTokens) return TV_ERR_UNSUPPORTED;
-  const W4Params p{a->x, a->x_sm, a->x_scale, static_cast<const uint32_t*>(a->qweight), a->q_sn, a->scales, a->s_sn,
-                   a->out, a->o_sm, a->rows, a->n, a->k, a->group};
+  if (a->q_sn < a->k / 8) return TV_ERR_SHAPE;
+  if (staged(a)) {
+    size_t need = 0;
+    tv_w4_workspace_size(a, &need);
+    if (!a->workspace || a->workspace_bytes < need) return TV_ERR_WORKSPACE;
+    if (!aligned16(a->workspace)) return TV_ERR_ALIGN;
+  }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a->out_dtype == TV_BF16)
-    return a->x_dtype == TV_E4M3 ? launch_w4<__nv_fp8_e4m3, __nv_bfloat16>(p, st)
-                                 : launch_w4<__nv_bfloat16, __nv_bfloat16>(p, st);
-  return a->x_dtype == TV_E4M3 ? launch_w4<__nv_fp8_e4m3, __half>(p, st) : launch_w4<__half, __half>(p, st);
+  return a->out_dtype == TV_BF16 ? launch_w4<__nv_bfloat16>(a, st) : launch_w4<__half>(a, st);
 }
 
 }  // extern "C"

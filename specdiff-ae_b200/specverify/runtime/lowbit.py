@@ -153,7 +153,7 @@ def w4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, *, x
     a.rows, a.n, a.k, a.group = rows, n, k, k // groups
     a.x, a.x_sm = x2.data_ptr(), x2.stride(0)
     a.x_scale = x_scale.data_ptr() if fp8 else None
-    a.qweight, a.q_sn = qweight.data_ptr(), qweight.stride(0)
+    a.qweight, a.q_sn = qweight.data_ptr(), qweight.stride(0) if n > 1 else k // 8
     a.scales, a.s_sn = scales.data_ptr(), scales.stride(0)
     a.out, a.o_sm = res.data_ptr(), o_sm
     lib = _lib.load()

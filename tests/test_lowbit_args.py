@@ -96,8 +96,16 @@ def test_w4_linear_checks(lib):
     for k in ("x", "qweight", "scales", "out"):
         assert call(**{k: None}) == -8, k
     assert call(x_dtype=3) == -8                                # e4m3 rows need their scales
-    assert call(qweight=FAKE + 4) == -3 and call(q_sn=33) == -3
+    assert call(qweight=FAKE + 4) == -3 and call(q_sn=33) == -3 and call(q_sn=28) == -1
+    assert call(k=(1 << 20) + 64, q_sn=1 << 20) == -7 and call(n=(1 << 27) + 1) == -7
+    # rows that TMA cannot read are staged: 8 bits, off the 16-byte grid, or overlapping
+    for kw in (dict(x_dtype=3, x_scale=FAKE), dict(x=FAKE + 2), dict(x_sm=260), dict(x_sm=0)):
+        assert call(**kw) == -5, kw
+        assert call(**kw, workspace=FAKE, workspace_bytes=4 * 256 * 2 - 1) == -5
+        assert call(**kw, workspace=FAKE + 8, workspace_bytes=1 << 20) == -3
     assert lib.tv_w4_linear(None, None) == -8
     n = ctypes.c_size_t(0)
-    assert lib.tv_w4_workspace_size(ctypes.byref(args()), ctypes.byref(n)) == 0
+    assert lib.tv_w4_workspace_size(ctypes.byref(args()), ctypes.byref(n)) == 0 and n.value == 0
+    assert lib.tv_w4_workspace_size(ctypes.byref(args(x_dtype=3)), ctypes.byref(n)) == 0 and n.value == 4 * 256 * 2
+    assert lib.tv_w4_workspace_size(ctypes.byref(args(rows=1, x_sm=0)), ctypes.byref(n)) == 0 and n.value == 0
     assert lib.tv_w4_workspace_size(None, ctypes.byref(n)) == -8
