@@ -4,19 +4,20 @@
 //
 // A CTA takes 128 weight rows (the M of tcgen05.mma, one TMEM lane each), up
 // to 128 tokens (its N) and a range of k.  The packed weights stream through a
-// shared-memory ring (TMA, 128 rows x 128 k = 8 KB a stage).  Eight warps, two
-// groups of four, turn them into 16-bit values, a thread its own weight row,
-// and write those straight into tensor memory, where the MMA reads its A
-// operand; x comes by TMA as the B operand in 64-k tiles.
+// shared-memory ring (TMA, 128 rows x 256 k = 16 KB a stage).  Eight warps, two
+// groups of four, turn them into 16-bit values, a thread one half of a stage
+// of its own weight row, and write those straight into tensor memory, where
+// the MMA reads its A operand; x comes by TMA as the B operand in tiles of
+// 128 k.
 //
 //   warp 0      weight producer (TMA)
 //   warp 1      MMA issuer, tensor-memory owner
 //   warp 2      x producer (TMA)
-//   warps 4-11  weights to 16 bits (group w / 4 - 1 takes every other stage),
-//               then the epilogue (TMEM lane quarter w mod 4)
+//   warps 4-11  weights to 16 bits (group w / 4 - 1 takes that half of every
+//               stage), then the epilogue (TMEM lane quarter w mod 4)
 //
-// Where there are fewer tiles than CTAs that fit the GPU, a cluster of up to 8
-// CTAs splits k; the partial sums meet in distributed shared memory and are
+// Where there are fewer tiles than CTAs that fit the GPU, a cluster of 2, 4 or
+// 8 CTAs splits k; the partial sums meet in distributed shared memory and are
 // added in rank order, so results do not depend on timing.
 //
 // Bound by HBM (the packed weights once) up to about 80 tokens, by the tensor
@@ -41,22 +42,23 @@ namespace cg = cooperative_groups;
 
 constexpr int kRows = 128;                   // weight rows per CTA
 constexpr int kMaxTokens = 128;              // tokens per CTA
-constexpr int kStageK = 128;                 // k per weight stage
-constexpr int kWStage = kRows * kStageK / 2; // 8 KB
+constexpr int kHalfK = 128;                  // k per x tile, A buffer and group step
+constexpr int kStageK = 2 * kHalfK;          // k per weight stage
+constexpr int kWStage = kRows * kStageK / 2; // 16 KB
 constexpr int kThreads = 384;
 constexpr int kDequantWarp = 4;              // first of the eight
-constexpr int kMaxStages = 12;
+constexpr int kMaxStages = 8;
 constexpr int kRing = 112 * 1024;            // both rings: two CTAs share an SM
 constexpr int kSmem = kRing + 1024;
 constexpr uint32_t kTmemCols = 256;          // two CTAs per SM
-constexpr uint32_t kACol = 128;              // accumulator in columns 0-127, four 32-column A buffers after it
+constexpr uint32_t kACol = 128;              // accumulator in columns 0-127, two 64-column A buffers after it
 constexpr int kMaxCluster = 8;
 constexpr int kSlots = 2 * kNumSMs;
 
 struct Bars {
   uint64_t w_full[kMaxStages], w_empty[kMaxStages];
   uint64_t x_full[kMaxStages], x_empty[kMaxStages];
-  uint64_t a_full[4], a_empty[4];
+  uint64_t a_full[2], a_empty[2];
   uint64_t done;
   uint32_t tmem;
   int abort;
@@ -73,6 +75,7 @@ struct W4Params {
   int tokens;                  // N of the MMA: tokens per CTA, a multiple of 16
   int w_stages, x_stages, x_bytes;
   int split;                   // CTAs of a cluster
+  uint32_t zero;               // 0, unknown to the compiler
   uint32_t group_magic;        // k / group = (k / 32) * magic >> 32; 0: group 32
 };
 
@@ -96,10 +99,10 @@ template <typename T> struct Unpack;
 template <> struct Unpack<__nv_bfloat16> {
   __nv_bfloat162 sa, sb, off;
   __device__ __forceinline__ void scale(__nv_bfloat16 s) {
-    const float f = __bfloat162float(s);
-    sa = __float2bfloat162_rn(f * 9.903520314283042e27f);      // 2^93
-    sb = __float2bfloat162_rn(f * 6.189700196426902e26f);      // 2^89
-    off = __float2bfloat162_rn(f * -7.275957614183426e-12f);   // -2^-37
+    const __nv_bfloat162 s2 = __halves2bfloat162(s, s);
+    sa = __hmul2(s2, __float2bfloat162_rn(9.903520314283042e27f));      // 2^93
+    sb = __hmul2(s2, __float2bfloat162_rn(6.189700196426902e26f));      // 2^89
+    off = __hmul2(s2, __float2bfloat162_rn(-7.275957614183426e-12f));   // -2^-37
   }
   __device__ __forceinline__ void word(uint32_t w, uint32_t* o) const {
     const uint32_t v = w >> 8;
@@ -137,7 +140,7 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* v) {
 __device__ __forceinline__ void drain(uint64_t* full, int stages, int it) {
   volatile int keep_waiting = 0;
   for (int j = it > stages ? it - stages : 0; j < it; ++j)
-    mbar_wait(&full[j % stages], (j / stages) & 1, &keep_waiting, 200000000ull);
+    mbar_wait_suspend(&full[j % stages], (j / stages) & 1, &keep_waiting, 400000000ll);
 }
 
 template <typename T>
@@ -146,7 +149,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   extern __shared__ __align__(1024) uint8_t smem[];
   Bars* bars = reinterpret_cast<Bars*>(smem + kRing);
   volatile int* abort = &bars->abort;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = blockIdx.x % p.split;
   const int n0 = blockIdx.x / p.split * kRows;
   const int t0 = blockIdx.y * p.tokens;
@@ -160,13 +163,13 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.w_stages; ++i) {
       mbar_init(&bars->w_full[i], 1);
-      mbar_init(&bars->w_empty[i], 4);
+      mbar_init(&bars->w_empty[i], 8);
     }
     for (int i = 0; i < p.x_stages; ++i) {
       mbar_init(&bars->x_full[i], 1);
       mbar_init(&bars->x_empty[i], 1);
     }
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&bars->a_full[i], 4);
       mbar_init(&bars->a_empty[i], 1);
     }
@@ -183,79 +186,75 @@ __global__ void __launch_bounds__(kThreads, 2)
   tc_fence_after();
   const uint32_t tmem = bars->tmem;
 
-  if (warp == 0) {
-    if (lane == 0) {
-      int s = 0, ph = 1, i = 0;
-      bool ok = true;
-      for (; i < nb; ++i) {
-        if (i >= p.w_stages && !mbar_wait(&bars->w_empty[s], ph, abort)) {
-          ok = false;
-          break;
-        }
-        mbar_arrive_expect_tx(&bars->w_full[s], kWStage);
-        tma_load_2d(w_ring + s * kWStage, &tmw, &bars->w_full[s], (kb0 + i) * (kStageK / 2), n0);
-        if (++s == p.w_stages) {
-          s = 0;
-          ph ^= 1;
+  if (warp == 0 || warp == 2) {
+    // ---- producers.  A thread keeps about one TMA box in flight, so a
+    // warp's lanes take turns issuing.
+    const bool wt = warp == 0;
+    uint64_t* full = wt ? bars->w_full : bars->x_full;
+    uint64_t* empty = wt ? bars->w_empty : bars->x_empty;
+    const int stages = wt ? p.w_stages : p.x_stages, count = wt ? nb : 2 * nb;
+    int s = 0, ph = 1, i = 0;
+    for (; i < count; ++i) {
+      if (i >= stages && !__all_sync(0xffffffffu, mbar_wait_suspend(&empty[s], ph, abort))) {
+        bars->abort = 1;
+        break;
+      }
+      if (lane == (i & 31)) {
+        if (wt) {
+          mbar_arrive_expect_tx(&full[s], kWStage);
+          tma_load_2d(w_ring + s * kWStage, &tmw, &full[s], (kb0 + i) * (kStageK / 2), n0);
+        } else {
+          mbar_arrive_expect_tx(&full[s], p.x_bytes);
+          tma_load_3d(x_ring + s * p.x_bytes, &tmx, &full[s], 0, t0, 4 * kb0 + 2 * i);
         }
       }
-      if (!ok) bars->abort = 1;
-      drain(bars->w_full, p.w_stages, i);
-    }
-  } else if (warp == 2) {
-    if (lane == 0) {
-      int s = 0, ph = 1, i = 0;
-      bool ok = true;
-      for (; i < 2 * nb; ++i) {
-        if (i >= p.x_stages && !mbar_wait(&bars->x_empty[s], ph, abort)) {
-          ok = false;
-          break;
-        }
-        mbar_arrive_expect_tx(&bars->x_full[s], p.x_bytes);
-        tma_load_2d(x_ring + s * p.x_bytes, &tmx, &bars->x_full[s], (2 * kb0 + i) * 64, t0);
-        if (++s == p.x_stages) {
-          s = 0;
-          ph ^= 1;
-        }
+      __syncwarp();
+      if (++s == stages) {
+        s = 0;
+        ph ^= 1;
       }
-      if (!ok) bars->abort = 1;
-      drain(bars->x_full, p.x_stages, i);
     }
+    if (lane == 0) drain(full, stages, i);
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-      const uint32_t idesc = idesc_f16(fmt, kRows, (uint32_t)p.tokens, 0);
-      int xs = 0, xph = 0;
-      bool ok = true;
-      for (int i = 0; ok && i < nb; ++i) {
-        for (int h = 0; h < 2; ++h) {
-          const int buf = (i & 1) * 2 + h;
-          if (!mbar_wait(&bars->x_full[xs], xph, abort) || !mbar_wait(&bars->a_full[buf], (i >> 1) & 1, abort)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t b = smem_u32(x_ring + xs * p.x_bytes);
-          const uint32_t a = tmem + kACol + (uint32_t)(buf * 32);
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_ts(tmem, a + kk * 8, smem_desc_sw128(b + kk * 32, 16, 1024), idesc, (i | h | kk) ? 1u : 0u);
-          tc_commit(&bars->a_empty[buf]);
-          tc_commit(&bars->x_empty[xs]);
-          if (++xs == p.x_stages) {
-            xs = 0;
-            xph ^= 1;
-          }
-        }
+    // ---- MMA issuer: the whole warp walks the loop, one elected lane issues
+    constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    const uint32_t idesc = idesc_f16(fmt, kRows, (uint32_t)p.tokens, 0);
+    const uint64_t desc0 = smem_desc_sw128(smem_u32(x_ring), 16, 1024);
+    const uint32_t half_tile = (uint32_t)p.x_bytes >> 5;          // 64 k of x, in descriptor units
+    const bool elected = elect_one();
+    int xs = 0, xph = 0;
+    bool ok = true;
+    for (int i = 0; i < 2 * nb; ++i) {
+      const int g = i & 1;
+      if (!mbar_wait_suspend(&bars->x_full[xs], xph, abort) ||
+          !mbar_wait_suspend(&bars->a_full[g], (i >> 1) & 1, abort)) {
+        ok = false;
+        break;
       }
-      if (ok) tc_commit(&bars->done);
-      else bars->abort = 1;
+      tc_fence_after();
+      const uint64_t b = desc0 + (uint32_t)((xs * p.x_bytes) >> 4);
+      const uint32_t a = tmem + kACol + (uint32_t)(g * 64);
+      if (elected) {
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          mma_ts(tmem, a + kk * 8, b + (kk >> 2) * half_tile + (kk & 3) * 2, idesc, (i | kk) ? 1u : 0u);
+        tc_commit(&bars->a_empty[g]);
+        tc_commit(&bars->x_empty[xs]);
+      }
+      __syncwarp();
+      if (++xs == p.x_stages) {
+        xs = 0;
+        xph ^= 1;
+      }
     }
+    if (!ok) bars->abort = 1;
+    else if (elected) tc_commit(&bars->done);
   } else if (warp >= kDequantWarp) {
     const int g = (warp - kDequantWarp) >> 2;
     const int q4 = warp & 3;
     const int r = q4 * 32 + lane;                        // weight row = TMEM lane
     const uint32_t lanes = tmem + ((uint32_t)(q4 * 32) << 16);
+    const uint32_t a_buf = lanes + kACol + (uint32_t)(g * 64);
     const T* srow = static_cast<const T*>(p.s) + (int64_t)min(n0 + r, p.n - 1) * p.s_sn;
     const int units = n0 + r < p.n ? p.k / 32 : 0;       // 32-k units of this row; scale 0 past the end
     auto scale_at = [&](int u) {
@@ -264,25 +263,29 @@ __global__ void __launch_bounds__(kThreads, 2)
     };
     T sc[4];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) sc[b] = scale_at((kb0 + g) * 4 + b);
-    int s = g, ph = 0;
+    for (int b = 0; b < 4; ++b) sc[b] = scale_at(kb0 * 8 + g * 4 + b);
+    int s = 0, ph = 0;
     bool ok = true;
-    for (int i = g; i < nb; i += 2) {
-      if (!__all_sync(0xffffffffu, mbar_wait(&bars->w_full[s], ph, abort))) {
+    for (int i = 0; i < nb; ++i) {
+      if (!__all_sync(0xffffffffu, mbar_wait_suspend(&bars->w_full[s], ph, abort))) {
         ok = false;
         break;
       }
       uint4 w[4];
-      const uint8_t* src = w_ring + s * kWStage + r * 64;
+      const uint8_t* src = w_ring + s * kWStage + r * 128;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) w[c] = *reinterpret_cast<const uint4*>(src + ((c ^ ((r >> 1) & 3)) << 4));
+      for (int c = 0; c < 4; ++c) w[c] = *reinterpret_cast<const uint4*>(src + (((g * 4 + c) ^ (r & 7)) << 4));
+      // Release the stage once the loads have come back: an arrival may pass
+      // loads that are still on their way, and the next TMA write with it, so
+      // its address is made to depend on a word of each (p.zero is 0).
+      const uint32_t seen = (w[0].x ^ w[1].x ^ w[2].x ^ w[3].x) & p.zero;
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->w_empty[s]);
+      if (lane == 0) mbar_arrive(&bars->w_empty[s] + seen);
       Unpack<T> un[4];
 #pragma unroll
       for (int b = 0; b < 4; ++b) un[b].scale(sc[b]);
 #pragma unroll
-      for (int b = 0; b < 4; ++b) sc[b] = scale_at((kb0 + i + 2) * 4 + b);
+      for (int b = 0; b < 4; ++b) sc[b] = scale_at((kb0 + i + 1) * 8 + g * 4 + b);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t o[32];
@@ -295,29 +298,29 @@ __global__ void __launch_bounds__(kThreads, 2)
           u.word(v.z, o + c * 16 + 8);
           u.word(v.w, o + c * 16 + 12);
         }
-        const int buf = g * 2 + h;
-        // the MMAs that read this buffer's previous contents have finished
-        if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait(&bars->a_empty[buf], ((i >> 1) & 1) ^ 1, abort))) {
-          ok = false;
-          break;
+        if (h == 0) {
+          // the MMAs that read this buffer's previous contents have finished
+          if (i >= 1 && !__all_sync(0xffffffffu, mbar_wait_suspend(&bars->a_empty[g], (i & 1) ^ 1, abort))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
         }
-        tc_fence_after();
-        tmem_st32(lanes + kACol + (uint32_t)(buf * 32), o);
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->a_full[buf]);
+        tmem_st32(a_buf + (uint32_t)(h * 32), o);
       }
       if (!ok) break;
-      s += 2;
-      if (s >= p.w_stages) {
-        s -= p.w_stages;
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->a_full[g]);
+      if (++s == p.w_stages) {
+        s = 0;
         ph ^= 1;
       }
     }
     if (!ok) bars->abort = 1;
     // ---- epilogue
-    ok = __all_sync(0xffffffffu, mbar_wait(&bars->done, 0, abort)) && ok;
+    ok = __all_sync(0xffffffffu, mbar_wait_suspend(&bars->done, 0, abort)) && ok;
     if (!ok) bars->abort = 1;
     tc_fence_after();
     T* out = static_cast<T*>(p.out);
@@ -368,31 +371,36 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 }
 
-// x that TMA cannot read (8 bits, or rows off the 16-byte grid) -> dense 16-bit
-// rows.  Both types hold every e4m3 value exactly.
+// x that TMA cannot read as it is -> dense 16-bit rows of a multiple of 64,
+// zeros behind k: 8-bit rows (both 16-bit types hold every e4m3 value exactly),
+// rows off the 16-byte grid, and rows that end inside a 64-k tile.
+__host__ __device__ constexpr int padded_k(int k) { return (k + 63) / 64 * 64; }
+
 template <typename X, typename T>
 __global__ void __launch_bounds__(256) w4_stage_kernel(const X* x, int64_t x_sm, T* y, int rows, int k) {
-  const int chunks = k / 8;
+  const int chunks = padded_k(k) / 8;
   const int64_t total = (int64_t)rows * chunks;
   for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
     const int64_t r = e / chunks;
     const int c = (int)(e - r * chunks) * 8;
     const X* src = x + r * x_sm + c;
-    float f[8];
-    if (sizeof(X) == 1 && (reinterpret_cast<uintptr_t>(src) & 7) == 0) {
-      const uint2 raw = *reinterpret_cast<const uint2*>(src);
-      const X* b = reinterpret_cast<const X*>(&raw);
+    float f[8] = {};
+    if (c < k) {
+      if (sizeof(X) == 1 && (reinterpret_cast<uintptr_t>(src) & 7) == 0) {
+        const uint2 raw = *reinterpret_cast<const uint2*>(src);
+        const X* b = reinterpret_cast<const X*>(&raw);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = static_cast<float>(b[i]);
-    } else {
+        for (int i = 0; i < 8; ++i) f[i] = static_cast<float>(b[i]);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = static_cast<float>(src[i]);
+        for (int i = 0; i < 8; ++i) f[i] = static_cast<float>(src[i]);
+      }
     }
     uint4 o;
     uint32_t* w = reinterpret_cast<uint32_t*>(&o);
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = Elem<T>::pack2(f[2 * i], f[2 * i + 1]);
-    *reinterpret_cast<uint4*>(y + r * k + c) = o;
+    *reinterpret_cast<uint4*>(y + r * padded_k(k) + c) = o;
   }
 }
 
@@ -409,29 +417,28 @@ PFN_cuTensorMapEncodeTiled_v12000 encoder() {
   return fn;
 }
 
-bool make_map(CUtensorMap* map, CUtensorMapDataType dt, CUtensorMapSwizzle swizzle, const void* base, uint64_t inner,
-              uint64_t outer, uint64_t stride_bytes, uint32_t box_inner, uint32_t box_outer) {
+bool make_map(CUtensorMap* map, CUtensorMapDataType dt, int dims, const void* base, const cuuint64_t* size,
+              const cuuint64_t* stride_bytes, const cuuint32_t* box) {
   auto enc = encoder();
-  if (!enc) return false;
-  cuuint64_t dims[2] = {inner, outer};
-  cuuint64_t strides[1] = {stride_bytes};
-  cuuint32_t box[2] = {box_inner, box_outer}, estr[2] = {1, 1};
-  return enc(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  const cuuint32_t one[3] = {1, 1, 1};
+  return enc && enc(map, dt, dims, const_cast<void*>(base), size, stride_bytes, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// TMA reads 16-bit rows on the 16-byte grid; one row needs no stride of its own.
+// Whether x goes through the staging copy; one row needs no stride of its own.
 bool staged(const tv_w4_args* a) {
-  return a->x_dtype == TV_E4M3 || !aligned16(a->x) || (a->rows > 1 && (a->x_sm < a->k || a->x_sm % 8 != 0));
+  return a->x_dtype == TV_E4M3 || a->k % 64 != 0 || !aligned16(a->x) ||
+         (a->rows > 1 && (a->x_sm < a->k || a->x_sm % 8 != 0));
 }
 
 template <typename T>
 int launch_w4(const tv_w4_args* a, cudaStream_t st) {
   const void* x = a->x;
-  int64_t x_sm = a->rows > 1 ? a->x_sm : a->k;
+  int64_t x_sm = a->rows > 1 ? a->x_sm : padded_k(a->k);
   if (staged(a)) {
     T* y = static_cast<T*>(a->workspace);
-    const int64_t chunks = (int64_t)a->rows * (a->k / 8);
+    const int64_t chunks = (int64_t)a->rows * (padded_k(a->k) / 8);
     const int blocks = (int)(chunks / 256 + 1 < 4 * kNumSMs ? chunks / 256 + 1 : 4 * kNumSMs);
     if (a->x_dtype == TV_E4M3)
       w4_stage_kernel<__nv_fp8_e4m3, T><<<blocks, 256, 0, st>>>(static_cast<const __nv_fp8_e4m3*>(a->x), a->x_sm, y,
@@ -441,7 +448,7 @@ int launch_w4(const tv_w4_args* a, cudaStream_t st) {
     const int rc = check_launch();
     if (rc != TV_OK) return rc;
     x = y;
-    x_sm = a->k;
+    x_sm = padded_k(a->k);
   }
   W4Params p{};
   p.s = a->scales;
@@ -453,26 +460,28 @@ int launch_w4(const tv_w4_args* a, cudaStream_t st) {
   p.n = a->n;
   p.k = a->k;
   p.tokens = a->rows >= kMaxTokens ? kMaxTokens : (a->rows + 15) / 16 * 16;
-  p.x_bytes = p.tokens * 128;
-  // rings: enough x tiles to cover an L2 round trip, the rest to the weights
-  p.x_stages = p.tokens <= 32 ? 8 : p.tokens <= 64 ? 6 : p.tokens <= 80 ? 5 : p.tokens <= 112 ? 4 : 3;
+  p.x_bytes = p.tokens * kHalfK * 2;
+  // rings: x tiles to cover an L2 round trip, the rest to the weights (3 to 5 stages)
+  p.x_stages = p.tokens <= 16 ? 6 : p.tokens <= 48 ? 4 : p.tokens <= 80 ? 3 : 2;
   p.w_stages = (kRing - p.x_stages * p.x_bytes) / kWStage;
-  if (p.w_stages > kMaxStages) p.w_stages = kMaxStages;
   const uint32_t g32 = (uint32_t)a->group / 32;
   p.group_magic = g32 == 1 ? 0 : (uint32_t)(((1ull << 32) + g32 - 1) / g32);
   const int blocks_t = (a->rows + p.tokens - 1) / p.tokens;
   const int64_t tiles = (int64_t)((a->n + kRows - 1) / kRows) * blocks_t;
   const int stages = (a->k + kStageK - 1) / kStageK;
   p.split = 1;
-  while (p.split < kMaxCluster && tiles * (p.split + 1) <= kSlots && stages >= 2 * (p.split + 1)) ++p.split;
+  while (p.split < kMaxCluster && tiles * p.split * 2 <= kSlots && stages >= p.split * 2) p.split *= 2;
   CUtensorMap mw, mx;
-  if (!make_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_64B, a->qweight, (uint64_t)a->k / 2,
-                (uint64_t)a->n, (uint64_t)a->q_sn * 4, kStageK / 2, kRows) ||
-      !make_map(&mx,
-                std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                                      : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                CU_TENSOR_MAP_SWIZZLE_128B, x, (uint64_t)a->k, (uint64_t)a->rows, (uint64_t)x_sm * 2, 64,
-                (uint32_t)p.tokens))
+  const cuuint64_t w_size[2] = {(cuuint64_t)a->k / 2, (cuuint64_t)a->n}, w_stride[1] = {(cuuint64_t)a->q_sn * 4};
+  const cuuint32_t w_box[2] = {kStageK / 2, kRows};
+  // x as [k / 64][rows][64]: one box is a 128-k tile, each 64 k of it 128-byte swizzled rows
+  const cuuint64_t x_size[3] = {64, (cuuint64_t)a->rows, (cuuint64_t)padded_k(a->k) / 64};
+  const cuuint64_t x_stride[2] = {(cuuint64_t)x_sm * 2, 128};
+  const cuuint32_t x_box[3] = {64, (cuuint32_t)p.tokens, kHalfK / 64};
+  const CUtensorMapDataType dt = std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                                       : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  if (!make_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, a->qweight, w_size, w_stride, w_box) ||
+      !make_map(&mx, dt, 3, x, x_size, x_stride, x_box))
     return TV_ERR_UNSUPPORTED;
   const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(w4_kernel<T>), kSmem);
   if (rc != TV_OK) return rc;
@@ -513,7 +522,7 @@ int tv_w4_workspace_size(const tv_w4_args* a, size_t* bytes) {
   if (!a || !bytes) return TV_ERR_NULL;
   const int rc = check_shape(a);
   if (rc != TV_OK) return rc;
-  *bytes = a->rows > 0 && staged(a) ? (size_t)a->rows * a->k * 2 : 0;
+  *bytes = a->rows > 0 && staged(a) ? (size_t)a->rows * padded_k(a->k) * 2 : 0;
   return TV_OK;
 }
 
