@@ -16,8 +16,8 @@
 //   warps 4-11  weights to 16 bits (group w / 4 - 1 takes that half of every
 //               stage), then the epilogue (TMEM lane quarter w mod 4)
 //
-// Where there are fewer tiles than CTAs that fit the GPU, a cluster of 2, 4 or
-// 8 CTAs splits k; the partial sums meet in distributed shared memory and are
+// Where there are fewer tiles than CTAs that fit the GPU, a cluster of up to 8
+// CTAs splits k; the partial sums meet in distributed shared memory and are
 // added in rank order, so results do not depend on timing.
 //
 // Bound by HBM (the packed weights once) up to about 80 tokens, by the tensor
@@ -53,7 +53,6 @@ constexpr int kSmem = kRing + 1024;
 constexpr uint32_t kTmemCols = 256;          // two CTAs per SM
 constexpr uint32_t kACol = 128;              // accumulator in columns 0-127, two 64-column A buffers after it
 constexpr int kMaxCluster = 8;
-constexpr int kSlots = 2 * kNumSMs;
 
 struct Bars {
   uint64_t w_full[kMaxStages], w_empty[kMaxStages];
@@ -71,7 +70,7 @@ struct W4Params {
   const float* x_scale;
   void* out;
   int64_t o_sm;
-  int rows, n, k;
+  int rows, n, k, groups;
   int tokens;                  // N of the MMA: tokens per CTA, a multiple of 16
   int w_stages, x_stages, x_bytes;
   int split;                   // CTAs of a cluster
@@ -98,8 +97,8 @@ template <typename T> __device__ __forceinline__ uint32_t as_bits(T v) { return 
 template <typename T> struct Unpack;
 template <> struct Unpack<__nv_bfloat16> {
   __nv_bfloat162 sa, sb, off;
-  __device__ __forceinline__ void scale(__nv_bfloat16 s) {
-    const __nv_bfloat162 s2 = __halves2bfloat162(s, s);
+  __device__ __forceinline__ void scale(uint32_t twice) {      // the scale's bits in both halves
+    const __nv_bfloat162 s2 = bits_as<__nv_bfloat162>(twice);
     sa = __hmul2(s2, __float2bfloat162_rn(9.903520314283042e27f));      // 2^93
     sb = __hmul2(s2, __float2bfloat162_rn(6.189700196426902e26f));      // 2^89
     off = __hmul2(s2, __float2bfloat162_rn(-7.275957614183426e-12f));   // -2^-37
@@ -115,7 +114,7 @@ template <> struct Unpack<__nv_bfloat16> {
 };
 template <> struct Unpack<__half> {
   __half2 s2;
-  __device__ __forceinline__ void scale(__half s) { s2 = __half2half2(s); }
+  __device__ __forceinline__ void scale(uint32_t twice) { s2 = bits_as<__half2>(twice); }
   __device__ __forceinline__ void word(uint32_t w, uint32_t* o) const {
     const uint32_t v = w >> 8;
     const __half2 lo = __float2half2_rn(-1032.f), sixteenth = __float2half2_rn(0.0625f), hi = __float2half2_rn(-72.f);
@@ -143,7 +142,13 @@ __device__ __forceinline__ void drain(uint64_t* full, int stages, int it) {
     mbar_wait_suspend(&full[j % stages], (j / stages) & 1, &keep_waiting, 400000000ll);
 }
 
-template <typename T>
+// A thread reads the scales of its own row, so a warp's load touches 32 rows:
+// 32 sectors however little of each it takes.  SCALES says how few loads do:
+//   0  group a multiple of 128, rows on the 16-byte grid: one scale a half
+//      stage, eight fetched at a time (one load in four stages at group 128)
+//   1, 2  group 32 or 64, rows on the 8- or 4-byte grid: one load a half stage
+//   3  anything else: each 32 k on its own
+template <typename T, int SCALES>
 __global__ void __launch_bounds__(kThreads, 2)
     w4_kernel(const __grid_constant__ CUtensorMap tmw, const __grid_constant__ CUtensorMap tmx, const W4Params p) {
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -160,24 +165,54 @@ __global__ void __launch_bounds__(kThreads, 2)
   uint8_t* w_ring = smem;
   uint8_t* x_ring = smem + p.w_stages * kWStage;
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < p.w_stages; ++i) {
-      mbar_init(&bars->w_full[i], 1);
-      mbar_init(&bars->w_empty[i], 8);
+  // ---- producers' state.  A thread keeps about one TMA box in flight, so a
+  // warp's lanes take turns issuing.
+  const bool wt = warp == 0;
+  uint64_t* full = wt ? bars->w_full : bars->x_full;
+  uint64_t* empty = wt ? bars->w_empty : bars->x_empty;
+  const int ring = wt ? p.w_stages : p.x_stages, count = wt ? nb : 2 * nb;
+  int pi = 0, ps = 0, pph = 1;
+  auto issue = [&] {
+    if (lane == (pi & 31)) {
+      if (wt) {
+        mbar_arrive_expect_tx(&full[ps], kWStage);
+        tma_load_2d(w_ring + ps * kWStage, &tmw, &full[ps], (kb0 + pi) * (kStageK / 2), n0);
+      } else {
+        mbar_arrive_expect_tx(&full[ps], p.x_bytes);
+        tma_load_3d(x_ring + ps * p.x_bytes, &tmx, &full[ps], 0, t0, 4 * kb0 + 2 * pi);
+      }
     }
-    for (int i = 0; i < p.x_stages; ++i) {
-      mbar_init(&bars->x_full[i], 1);
-      mbar_init(&bars->x_empty[i], 1);
+    __syncwarp();
+    if (++ps == ring) {
+      ps = 0;
+      pph ^= 1;
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&bars->a_full[i], 4);
-      mbar_init(&bars->a_empty[i], 1);
+    ++pi;
+  };
+  if (wt || warp == 2) {
+    // each producer sets up its own barriers and fills its ring before the
+    // CTA meets: the first loads run while tensor memory is allocated
+    if (lane == 0) {
+      prefetch_tmap(wt ? &tmw : &tmx);
+      for (int i = 0; i < ring; ++i) {
+        mbar_init(&full[i], 1);
+        mbar_init(&empty[i], wt ? 8 : 1);
+      }
+      mbar_fence_init();
     }
-    mbar_init(&bars->done, 1);
-    bars->abort = 0;
-    mbar_fence_init();
-  }
-  if (warp == 1) {
+    __syncwarp();
+    while (pi < count && pi < ring) issue();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&bars->a_full[i], 4);
+        mbar_init(&bars->a_empty[i], 1);
+      }
+      mbar_init(&bars->done, 1);
+      bars->abort = 0;
+      mbar_fence_init();
+    }
+    __syncwarp();
     tmem_alloc(&bars->tmem, kTmemCols);
     tmem_relinquish();
   }
@@ -186,35 +221,15 @@ __global__ void __launch_bounds__(kThreads, 2)
   tc_fence_after();
   const uint32_t tmem = bars->tmem;
 
-  if (warp == 0 || warp == 2) {
-    // ---- producers.  A thread keeps about one TMA box in flight, so a
-    // warp's lanes take turns issuing.
-    const bool wt = warp == 0;
-    uint64_t* full = wt ? bars->w_full : bars->x_full;
-    uint64_t* empty = wt ? bars->w_empty : bars->x_empty;
-    const int stages = wt ? p.w_stages : p.x_stages, count = wt ? nb : 2 * nb;
-    int s = 0, ph = 1, i = 0;
-    for (; i < count; ++i) {
-      if (i >= stages && !__all_sync(0xffffffffu, mbar_wait_suspend(&empty[s], ph, abort))) {
+  if (wt || warp == 2) {
+    while (pi < count) {
+      if (!__all_sync(0xffffffffu, mbar_wait_suspend(&empty[ps], pph, abort))) {
         bars->abort = 1;
         break;
       }
-      if (lane == (i & 31)) {
-        if (wt) {
-          mbar_arrive_expect_tx(&full[s], kWStage);
-          tma_load_2d(w_ring + s * kWStage, &tmw, &full[s], (kb0 + i) * (kStageK / 2), n0);
-        } else {
-          mbar_arrive_expect_tx(&full[s], p.x_bytes);
-          tma_load_3d(x_ring + s * p.x_bytes, &tmx, &full[s], 0, t0, 4 * kb0 + 2 * i);
-        }
-      }
-      __syncwarp();
-      if (++s == stages) {
-        s = 0;
-        ph ^= 1;
-      }
+      issue();
     }
-    if (lane == 0) drain(full, stages, i);
+    if (lane == 0) drain(full, ring, pi);
   } else if (warp == 1) {
     // ---- MMA issuer: the whole warp walks the loop, one elected lane issues
     constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
@@ -255,15 +270,59 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int r = q4 * 32 + lane;                        // weight row = TMEM lane
     const uint32_t lanes = tmem + ((uint32_t)(q4 * 32) << 16);
     const uint32_t a_buf = lanes + kACol + (uint32_t)(g * 64);
-    const T* srow = static_cast<const T*>(p.s) + (int64_t)min(n0 + r, p.n - 1) * p.s_sn;
-    const int units = n0 + r < p.n ? p.k / 32 : 0;       // 32-k units of this row; scale 0 past the end
-    auto scale_at = [&](int u) {
-      if (u >= units) return Elem<T>::from_f(0.f);
-      return srow[p.group_magic ? __umulhi((uint32_t)u, p.group_magic) : (uint32_t)u];
+    const T* row = static_cast<const T*>(p.s) + (int64_t)min(n0 + r, p.n - 1) * p.s_sn;
+    const int last = p.k / 32 - 1;                       // last 32-k unit
+    auto index = [&](int u) { return p.group_magic ? __umulhi((uint32_t)u, p.group_magic) : (uint32_t)u; };
+    constexpr int NS = SCALES == 0 ? 1 : SCALES == 2 ? 2 : 4;     // scales of a half row of a stage
+    // The bits that hold the scales of stage st, loaded one stage ahead
+    // and only taken apart there, so nothing waits for a load in flight.  Past
+    // the end of the weight they are those of its last row (not stored) and
+    // last group (its x is zero).
+    struct Raw {
+      uint32_t v[4];
     };
-    T sc[4];
+    auto load_scales = [&](int st, Raw& o) {
+      if constexpr (SCALES == 0) {
+        const T* at = row + (index(min(st * 8 + g * 4, last)) & ~7u);
+        // the last eight of a row that does not end on eight
+        if (at + 8 <= row + p.groups)
+          asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(o.v[0]), "=r"(o.v[1]), "=r"(o.v[2]), "=r"(o.v[3]) : "l"(at));
+        else {
+          for (int j = 0; j < 4; ++j) {
+            const uint16_t lo = 2 * j < row + p.groups - at ? reinterpret_cast<const uint16_t*>(at)[2 * j] : 0;
+            const uint16_t hi = 2 * j + 1 < row + p.groups - at ? reinterpret_cast<const uint16_t*>(at)[2 * j + 1] : 0;
+            o.v[j] = (uint32_t)hi << 16 | lo;
+          }
+        }
+      } else if constexpr (SCALES == 1) {
+        const T* at = row + min(st * 8 + g * 4, (last / 4) * 4);
+        asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(o.v[0]), "=r"(o.v[1]) : "l"(at));
+      } else if constexpr (SCALES == 2) {
+        const T* at = row + min(st * 4 + g * 2, (last / 4) * 2);
+        asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(o.v[0]) : "l"(at));
+      } else {
 #pragma unroll
-    for (int b = 0; b < 4; ++b) sc[b] = scale_at(kb0 * 8 + g * 4 + b);
+        for (int b = 0; b < 4; ++b) {
+          const T* at = row + index(min(st * 8 + g * 4 + b, last));
+          asm volatile("{\n\t.reg .u16 t;\n\tld.global.nc.u16 t, [%1];\n\tcvt.u32.u16 %0, t;\n\t}" : "=r"(o.v[b]) : "l"(at));
+        }
+      }
+    };
+    // scale b of the half stage, its bits in both halves
+    auto scale_of = [&](const Raw& o, int st, int b) -> uint32_t {
+      if constexpr (SCALES == 0) {
+        const int u = min(st * 8 + g * 4, last);
+        const uint32_t i = index(u) & 7;
+        const uint32_t w = (i & 4) ? ((i & 2) ? o.v[3] : o.v[2]) : ((i & 2) ? o.v[1] : o.v[0]);
+        return __byte_perm(w, w, (i & 1) ? 0x3232 : 0x1010);
+      } else if constexpr (SCALES == 1 || SCALES == 2) {
+        return __byte_perm(o.v[b >> 1], 0, (b & 1) ? 0x3232 : 0x1010);
+      } else {
+        return o.v[b] * 0x10001u;
+      }
+    };
+    Raw raw;
+    load_scales(kb0, raw);
     int s = 0, ph = 0;
     bool ok = true;
     for (int i = 0; i < nb; ++i) {
@@ -281,17 +340,18 @@ __global__ void __launch_bounds__(kThreads, 2)
       const uint32_t seen = (w[0].x ^ w[1].x ^ w[2].x ^ w[3].x) & p.zero;
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->w_empty[s] + seen);
-      Unpack<T> un[4];
+      Unpack<T> un[NS];
 #pragma unroll
-      for (int b = 0; b < 4; ++b) un[b].scale(sc[b]);
-#pragma unroll
-      for (int b = 0; b < 4; ++b) sc[b] = scale_at((kb0 + i + 1) * 8 + g * 4 + b);
+      for (int b = 0; b < NS; ++b) un[b].scale(scale_of(raw, kb0 + i, b));
+      // eight scales at once last until their index leaves the eight
+      const int u = (kb0 + i + 1) * 8 + g * 4;
+      if (SCALES != 0 || ((index(u) ^ index(u - 8)) & ~7u)) load_scales(kb0 + i + 1, raw);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t o[32];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const Unpack<T>& u = un[h * 2 + c];
+          const Unpack<T>& u = un[NS == 1 ? 0 : NS == 2 ? h : h * 2 + c];
           const uint4 v = w[h * 2 + c];
           u.word(v.x, o + c * 16);
           u.word(v.y, o + c * 16 + 4);
@@ -330,14 +390,17 @@ __global__ void __launch_bounds__(kThreads, 2)
       uint32_t v[16];
       tmem_ld16(lanes + (uint32_t)(c * 16), v);
       tmem_wait_ld();
+      const int t = t0 + c * 16;
+      T* at = out + (int64_t)t * p.o_sm + n0 + r;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        const int t = t0 + c * 16 + j;
-        float f = __uint_as_float(v[j]) * Unpack<T>::unscale();
-        if (!ok) f = __int_as_float(0x7fc00000);
-        if (p.split > 1) part[(c * 16 + j) * kRows + r] = f;
-        else if (t < p.rows && n0 + r < p.n)
-          out[(int64_t)t * p.o_sm + n0 + r] = Elem<T>::from_f(p.x_scale ? f * p.x_scale[t] : f);
+        float f = ok ? __uint_as_float(v[j]) * Unpack<T>::unscale() : __int_as_float(0x7fc00000);
+        if (p.split > 1) {
+          part[(c * 16 + j) * kRows + r] = f;
+        } else if (t + j < p.rows && n0 + r < p.n) {
+          if (p.x_scale) f *= __ldg(p.x_scale + t + j);
+          at[j * p.o_sm] = Elem<T>::from_f(f);
+        }
       }
     }
   }
@@ -355,8 +418,11 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int j = rank + p.split * (tid / kRows); j < p.tokens; j += 2 * p.split) {
         const int t = t0 + j;
         if (t >= p.rows || n0 + r >= p.n) continue;
-        float f = 0.f;
-        for (int k = 0; k < p.split; ++k) f += *cluster.map_shared_rank(part + j * kRows + r, k);
+        float v[kMaxCluster], f = 0.f;
+#pragma unroll
+        for (int k = 0; k < kMaxCluster; ++k) v[k] = k < p.split ? *cluster.map_shared_rank(part + j * kRows + r, k) : 0.f;
+#pragma unroll
+        for (int k = 0; k < kMaxCluster; ++k) f += v[k];
         if (gave_up) f = __int_as_float(0x7fc00000);
         out[(int64_t)t * p.o_sm + n0 + r] = Elem<T>::from_f(p.x_scale ? f * p.x_scale[t] : f);
       }
@@ -432,6 +498,27 @@ bool staged(const tv_w4_args* a) {
          (a->rows > 1 && (a->x_sm < a->k || a->x_sm % 8 != 0));
 }
 
+template <typename T, int SCALES>
+int launch_kernel(const CUtensorMap& mw, const CUtensorMap& mx, const W4Params& p, int blocks_n, int blocks_t,
+                  cudaStream_t st) {
+  const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(w4_kernel<T, SCALES>), kSmem);
+  if (rc != TV_OK) return rc;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(blocks_n * p.split), (unsigned)blocks_t);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = p.split;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = p.split > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, w4_kernel<T, SCALES>, mw, mx, p);
+  return e == cudaSuccess ? check_launch() : record_cuda_error(e);
+}
+
 template <typename T>
 int launch_w4(const tv_w4_args* a, cudaStream_t st) {
   const void* x = a->x;
@@ -459,6 +546,7 @@ int launch_w4(const tv_w4_args* a, cudaStream_t st) {
   p.rows = a->rows;
   p.n = a->n;
   p.k = a->k;
+  p.groups = a->k / a->group;
   p.tokens = a->rows >= kMaxTokens ? kMaxTokens : (a->rows + 15) / 16 * 16;
   p.x_bytes = p.tokens * kHalfK * 2;
   // rings: x tiles to cover an L2 round trip, the rest to the weights (3 to 5 stages)
@@ -469,8 +557,13 @@ int launch_w4(const tv_w4_args* a, cudaStream_t st) {
   const int blocks_t = (a->rows + p.tokens - 1) / p.tokens;
   const int64_t tiles = (int64_t)((a->n + kRows - 1) / kRows) * blocks_t;
   const int stages = (a->k + kStageK - 1) / kStageK;
+  // the largest cluster of which that many run at once, two CTAs per SM (half
+  // of these pairs as the occupancy query reports them: clusters do not span
+  // processor groups)
+  constexpr int fit[kMaxCluster + 1] = {0, 296, 148, 90, 66, 52, 44, 30, 30};
   p.split = 1;
-  while (p.split < kMaxCluster && tiles * p.split * 2 <= kSlots && stages >= p.split * 2) p.split *= 2;
+  for (int c = 2; c <= kMaxCluster; ++c)
+    if (tiles <= fit[c] && stages >= c) p.split = c;
   CUtensorMap mw, mx;
   const cuuint64_t w_size[2] = {(cuuint64_t)a->k / 2, (cuuint64_t)a->n}, w_stride[1] = {(cuuint64_t)a->q_sn * 4};
   const cuuint32_t w_box[2] = {kStageK / 2, kRows};
@@ -483,22 +576,16 @@ int launch_w4(const tv_w4_args* a, cudaStream_t st) {
   if (!make_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, a->qweight, w_size, w_stride, w_box) ||
       !make_map(&mx, dt, 3, x, x_size, x_stride, x_box))
     return TV_ERR_UNSUPPORTED;
-  const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(w4_kernel<T>), kSmem);
-  if (rc != TV_OK) return rc;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((a->n + kRows - 1) / kRows * p.split), (unsigned)blocks_t);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kSmem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = p.split;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, w4_kernel<T>, mw, mx, p);
-  return e == cudaSuccess ? check_launch() : record_cuda_error(e);
+  const int blocks_n = (a->n + kRows - 1) / kRows;
+  // SCALES by what the layout allows; k a multiple of 128 keeps a half stage's
+  // load inside the row
+  auto grid_of = [&](int bytes) {
+    return reinterpret_cast<uintptr_t>(a->scales) % bytes == 0 && (a->n == 1 || a->s_sn * 2 % bytes == 0);
+  };
+  if (a->group % kHalfK == 0 && grid_of(16)) return launch_kernel<T, 0>(mw, mx, p, blocks_n, blocks_t, st);
+  if (a->group == 32 && a->k % kHalfK == 0 && grid_of(8)) return launch_kernel<T, 1>(mw, mx, p, blocks_n, blocks_t, st);
+  if (a->group == 64 && a->k % kHalfK == 0 && grid_of(4)) return launch_kernel<T, 2>(mw, mx, p, blocks_n, blocks_t, st);
+  return launch_kernel<T, 3>(mw, mx, p, blocks_n, blocks_t, st);
 }
 
 int check_shape(const tv_w4_args* a) {

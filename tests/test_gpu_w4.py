@@ -58,7 +58,10 @@ def check(y, x, q, s, xs=None):
 
 SHAPES = [(1, 64, 256, 128), (1, 6144, 4096, 128), (8, 1000, 704, 32), (17, 129, 1024, 64), (65, 4096, 4096, 128),
           (33, 4099, 14336, 32), (128, 2048, 896, 128), (129, 300, 512, 64), (300, 257, 96, 96), (3, 1, 32, 32),
-          (2, 7, 64, 64), (5, 127, 14336, 128), (16, 512, 160, 32), (80, 513, 2080, 32)]
+          (2, 7, 64, 64), (5, 127, 14336, 128), (16, 512, 160, 32), (80, 513, 2080, 32),
+          # many tiles: equal runs that cross tiles, rings that wrap; and two token blocks of them
+          (48, 40960, 4096, 128), (16, 28672, 4096, 64), (128, 25700, 1056, 32), (200, 13000, 768, 128),
+          (1, 40000, 256, 256)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])

@@ -103,6 +103,7 @@ def test_w4_linear_checks(lib):
         assert call(**kw) == -5, kw
         assert call(**kw, workspace=FAKE, workspace_bytes=4 * 256 * 2 - 1) == -5
         assert call(**kw, workspace=FAKE + 8, workspace_bytes=1 << 20) == -3
+    assert call(rows=65535 * 128 + 1) == -7
     assert lib.tv_w4_linear(None, None) == -8
     n = ctypes.c_size_t(0)
     assert lib.tv_w4_workspace_size(ctypes.byref(args()), ctypes.byref(n)) == 0 and n.value == 0
