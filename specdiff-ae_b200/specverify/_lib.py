@@ -230,11 +230,16 @@ def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def launch(dev: torch.device, fn, *args) -> int:
     """``fn(*args, stream)`` on ``dev``'s current stream, with ``dev`` current
     for the call (a kernel launches on the current device, not its tensors')."""
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    if dev.index == torch.cuda.current_device():
+    index = dev.index
+    # the stream's handle without the Stream object around it: 2 us less a call
+    stream = _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
+    if index == torch.cuda.current_device():
         return fn(*args, stream)
     with torch.cuda.device(dev):
         return fn(*args, stream)

@@ -206,50 +206,69 @@ def accept_residual(logits: torch.Tensor, draft: torch.Tensor, parent: torch.Ten
     node and -1 elsewhere.  Invalid values in a sequence (parents, drafted
     tokens, a row without a finite logit) are reported by ``to_host``.
     """
-    dev = _lib.require_cuda(logits, draft, parent, uniform, draft_probs, counts)
     single = logits.dim() == 2
-    lead = (1,) if single else tuple(logits.shape[:1])
-    if logits.dim() != (2 if single else 3) or logits.shape[-2] < 1 or logits.shape[-1] < 1:
+    shape = logits.shape
+    own = shape[:-2]
+    m, v = shape[-2:] if len(shape) >= 2 else (0, 0)
+    b = 1 if single else shape[0]
+    # one look at what every call has right; the exact complaint is looked for when it is not
+    if not (logits.is_cuda and 2 <= len(shape) <= 3 and m > 1 and v > 1 and logits.stride()[-1] == 1
+            and logits.dtype in _LOGITS and draft.shape == shape[:-1] == uniform.shape
+            and parent.shape == own + (m - 1,) and draft.dtype is parent.dtype is torch.int64
+            and uniform.dtype is torch.float32 and draft.stride()[-1] == uniform.stride()[-1] == 1
+            and (m == 2 or parent.stride()[-1] == 1)
+            and (draft_probs is None or (draft_probs.shape == shape and draft_probs.stride()[-1] == 1
+                                         and draft_probs.dtype in _LOGITS and draft_probs.device == logits.device))
+            and counts is None and logits.device == draft.device == parent.device == uniform.device):
+        _check_accept_residual(logits, draft, parent, uniform, draft_probs, counts)
+    code = _LOGITS[logits.dtype]
+    nxt = draft.new_empty(own + (m,))
+    res = draft.new_empty(own + (RESULT_HEADER + 2 * m,))
+    a = _lib.ResidualAcceptArgs(
+        code, b, m, v, logits.data_ptr(), 0 if single else logits.stride(0), logits.stride(-2),
+        draft.data_ptr(), 0 if single else draft.stride(0), parent.data_ptr(), 0 if single else parent.stride(0),
+        counts.data_ptr() if counts is not None else None, uniform.data_ptr(), 0 if single else uniform.stride(0))
+    if draft_probs is not None:
+        a.probs_dtype, a.probs = _LOGITS[draft_probs.dtype], draft_probs.data_ptr()
+        a.probs_sb, a.probs_sm = 0 if single else draft_probs.stride(0), draft_probs.stride(-2)
+    a.temperature, a.next_tokens, a.result = temperature, nxt.data_ptr(), res.data_ptr()
+    lib = _lib.load()
+    need = ctypes.c_size_t(0)
+    st = lib.tv_residual_accept_workspace_size(a, need)
+    if st == 0:
+        ws = logits.new_empty(need.value, dtype=torch.uint8)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need.value
+        st = _lib.launch(logits.device, lib.tv_residual_accept, a)
+    if st != 0:
+        _lib.check(st, "tv_residual_accept")
+    return AcceptResult(nxt, res, m)
+
+
+_LOGITS = {torch.bfloat16: _lib.TV_BF16, torch.float16: _lib.TV_F16, torch.float32: _lib.TV_F32}
+
+
+def _check_accept_residual(logits, draft, parent, uniform, draft_probs, counts) -> None:
+    _lib.require_cuda(logits, draft, parent, uniform, draft_probs, counts)
+    if logits.dim() not in (2, 3) or logits.shape[-2] < 1 or logits.shape[-1] < 1:
         raise _lib.SpecVerifyError(-1, f"logits must be [M, V] or [B, M, V], got {tuple(logits.shape)}")
-    m, v = logits.shape[-2], logits.shape[-1]
-    b = lead[0]
-    own = () if single else lead
+    m, v = logits.shape[-2:]
+    own = tuple(logits.shape[:-2])
+    if logits.dtype not in _LOGITS:
+        raise _lib.SpecVerifyError(-2, f"logits {logits.dtype} must be bfloat16, float16 or float32")
     for what, t, shape, dtype in (("draft", draft, own + (m,), torch.int64), ("parent", parent, own + (m - 1,), torch.int64),
-                                  ("uniform", uniform, own + (m,), torch.float32), ("counts", counts, (b,), torch.int32),
+                                  ("uniform", uniform, own + (m,), torch.float32),
+                                  ("counts", counts, own or (1,), torch.int32),
                                   ("draft_probs", draft_probs, own + (m, v), None)):
         if t is None:
             continue
         if tuple(t.shape) != shape:
             raise _lib.SpecVerifyError(-1, f"{what} must be {list(shape)}, got {list(t.shape)}")
-        if dtype is not None and t.dtype != dtype:
-            raise _lib.SpecVerifyError(-2, f"{what} must be {dtype}, got {t.dtype}")
+        if t.dtype != dtype if dtype is not None else t.dtype not in _LOGITS:
+            raise _lib.SpecVerifyError(-2, f"{what} must be {dtype or 'bfloat16, float16 or float32'}, got {t.dtype}")
         if t.shape[-1] > 1 and t.stride(-1) != 1:
             raise _lib.SpecVerifyError(-3, f"{what} must have unit stride on its last dimension")
     if v > 1 and logits.stride(-1) != 1:
         raise _lib.SpecVerifyError(-3, "logits must have unit stride on the vocabulary")
-    a = _lib.ResidualAcceptArgs()
-    a.logits_dtype, a.batch, a.rows, a.vocab = _lib.dtype_code(logits.dtype), b, m, v
-    a.logits, a.logits_sb, a.logits_sm = logits.data_ptr(), 0 if single else logits.stride(0), logits.stride(-2)
-    a.draft, a.draft_sb = draft.data_ptr(), 0 if single else draft.stride(0)
-    a.parent, a.parent_sb = parent.data_ptr(), 0 if single else parent.stride(0)
-    a.uniform, a.uniform_sb = uniform.data_ptr(), 0 if single else uniform.stride(0)
-    if counts is not None:
-        a.counts = counts.data_ptr()
-    if draft_probs is not None:
-        a.probs_dtype, a.probs = _lib.dtype_code(draft_probs.dtype), draft_probs.data_ptr()
-        a.probs_sb, a.probs_sm = 0 if single else draft_probs.stride(0), draft_probs.stride(-2)
-    a.temperature = float(temperature)
-    nxt = torch.empty(own + (m,), dtype=torch.int64, device=dev)
-    res = torch.empty(own + (RESULT_HEADER + 2 * m,), dtype=torch.int64, device=dev)
-    a.next_tokens, a.result = nxt.data_ptr(), res.data_ptr()
-    lib = _lib.load()
-    need = ctypes.c_size_t(0)
-    _lib.check(lib.tv_residual_accept_workspace_size(ctypes.byref(a), ctypes.byref(need)),
-               "tv_residual_accept_workspace_size")
-    ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), need.value
-    _lib.check(_lib.launch(dev, lib.tv_residual_accept, ctypes.byref(a)), "tv_residual_accept")
-    return AcceptResult(nxt, res, m)
 
 
 def accept_from_hidden(hidden: torch.Tensor, lm_head_weight: torch.Tensor, draft: Optional[torch.Tensor],

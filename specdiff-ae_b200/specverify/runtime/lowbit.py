@@ -18,7 +18,7 @@ from .. import _lib
 
 __all__ = ["add_rms_norm", "dequantize_w4", "quantize_w4", "w4_linear"]
 
-_HALF = (torch.bfloat16, torch.float16)
+_HALF = {torch.bfloat16: _lib.TV_BF16, torch.float16: _lib.TV_F16}
 
 
 def _rows_ok(t: torch.Tensor, shape, dtype, what: str) -> None:
@@ -42,7 +42,31 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, 
     scale 0 for a row of zeros, NaN for a row with a NaN).  ``h`` is written to
     ``residual_out`` when given, which may be ``residual`` itself.
     """
-    dev = _lib.require_cuda(x, residual, weight, residual_out)
+    shape, dtype = x.shape, x.dtype
+    # one look at what every call has right; the exact complaint is looked for when it is not
+    if not (x.is_cuda and len(shape) == 2 and dtype in _HALF and x.stride()[1] == 1 and residual.shape == shape
+            and residual.stride()[1] == 1 and residual.dtype is dtype and weight.dtype is dtype
+            and weight.shape == shape[1:] and weight.stride()[0] == 1 and residual.device == x.device == weight.device
+            and residual_out is None):
+        _check_add_rms_norm(x, residual, weight, residual_out)
+    rows, cols = shape
+    h = torch.empty_like(x, memory_format=torch.contiguous_format) if residual_out is None else residual_out
+    if fp8:
+        y = torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format)
+        scale = x.new_empty(rows, dtype=torch.float32)
+        scale_ptr = scale.data_ptr()
+    else:
+        y, scale_ptr = torch.empty_like(x, memory_format=torch.contiguous_format), None
+    st = _lib.launch(x.device, _lib.load().tv_add_rms_norm, x.data_ptr(), x.stride(0), residual.data_ptr(),
+                     residual.stride(0), weight.data_ptr(), h.data_ptr(), h.stride(0), y.data_ptr(), cols, scale_ptr,
+                     rows, cols, eps, _HALF[dtype])
+    if st != 0:
+        _lib.check(st, "tv_add_rms_norm")
+    return (y, scale, h) if fp8 else (y, h)
+
+
+def _check_add_rms_norm(x, residual, weight, residual_out) -> None:
+    _lib.require_cuda(x, residual, weight, residual_out)
     if x.dim() != 2:
         raise _lib.SpecVerifyError(-1, f"x must be [rows, cols], got {tuple(x.shape)}")
     if x.dtype not in _HALF:
@@ -53,20 +77,10 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, 
     if weight.shape != (cols,) or weight.dtype != x.dtype or (cols > 1 and weight.stride(0) != 1):
         raise _lib.SpecVerifyError(-1, f"weight must be a dense [{cols}] {x.dtype}, got {tuple(weight.shape)} "
                                        f"{weight.dtype}")
-    if residual_out is None:
-        residual_out = torch.empty((rows, cols), dtype=x.dtype, device=dev)
-    else:
+    if residual_out is not None:
         _rows_ok(residual_out, x.shape, x.dtype, "residual_out")
         if rows > 1 and residual_out.stride(0) < cols:
             raise _lib.SpecVerifyError(-1, f"residual_out's rows overlap (stride {residual_out.stride(0)})")
-    y = torch.empty((rows, cols), dtype=torch.float8_e4m3fn if fp8 else x.dtype, device=dev)
-    scale = torch.empty(rows, dtype=torch.float32, device=dev) if fp8 else None
-    st = _lib.launch(dev, _lib.load().tv_add_rms_norm, x.data_ptr(), x.stride(0), residual.data_ptr(),
-                     residual.stride(0), weight.data_ptr(), residual_out.data_ptr(), residual_out.stride(0),
-                     y.data_ptr(), cols, scale.data_ptr() if fp8 else None, rows, cols, float(eps),
-                     _lib.TV_BF16 if x.dtype == torch.bfloat16 else _lib.TV_F16)
-    _lib.check(st, "tv_add_rms_norm")
-    return (y, scale, residual_out) if fp8 else (y, residual_out)
 
 
 # nibble i of a packed word holds weight 8 c + _ORDER[i]
@@ -117,7 +131,41 @@ def w4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, *, x
     32).  Returns [..., N] in the scales' type, summed in fp32; ``out``, when
     given, is [rows, N] with unit stride on N.
     """
-    dev = _lib.require_cuda(x, qweight, scales, x_scale, out)
+    n, words = qweight.shape if qweight.dim() == 2 else (0, 0)
+    k, fp8 = words * 8, x.dtype is torch.float8_e4m3fn
+    groups = scales.shape[-1]
+    if not (x.is_cuda and x.dim() == 2 and x.shape[1] == k and x.stride()[1] == 1 and scales.dim() == 2
+            and scales.shape[0] == n > 1 and qweight.dtype is torch.int32 and scales.dtype in _HALF
+            and qweight.stride()[1] == 1 and scales.stride()[1] == 1 and (x.dtype is scales.dtype if not fp8 else False)
+            and x_scale is None and out is None and groups and k % (32 * groups) == 0
+            and x.device == qweight.device == scales.device):
+        _check_w4_linear(x, qweight, scales, x_scale, out)
+    x2 = x if x.dim() == 2 else x.reshape(-1, k)
+    rows = x2.shape[0]
+    if out is None:
+        res = scales.new_empty((rows, n) if x.dim() == 2 else x.shape[:-1] + (n,))
+        o_sm = n
+    else:
+        res, o_sm = out, out.stride(0)
+    kind = _HALF[scales.dtype]
+    a = _lib.W4Args(_lib.TV_E4M3 if fp8 else kind, kind, rows, n, k, k // groups, x2.data_ptr(), x2.stride(0),
+                    x_scale.data_ptr() if fp8 else None, qweight.data_ptr(), qweight.stride(0) if n > 1 else words,
+                    scales.data_ptr(), scales.stride(0), res.data_ptr(), o_sm)
+    lib = _lib.load()
+    need = ctypes.c_size_t(0)
+    st = lib.tv_w4_workspace_size(a, need)
+    if st == 0:
+        if need.value:
+            ws = x.new_empty(need.value, dtype=torch.uint8)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), need.value
+        st = _lib.launch(x.device, lib.tv_w4_linear, a)
+    if st != 0:
+        _lib.check(st, "tv_w4_linear")
+    return res
+
+
+def _check_w4_linear(x, qweight, scales, x_scale, out) -> None:
+    _lib.require_cuda(x, qweight, scales, x_scale, out)
     if x.dim() < 1 or qweight.dim() != 2 or scales.dim() != 2 or qweight.shape[0] != scales.shape[0]:
         raise _lib.SpecVerifyError(-1, f"x {tuple(x.shape)}, qweight {tuple(qweight.shape)}, scales "
                                        f"{tuple(scales.shape)}")
@@ -133,34 +181,11 @@ def w4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, *, x
         raise _lib.SpecVerifyError(-2, f"x {x.dtype} must be {scales.dtype} or float8_e4m3fn")
     if fp8 != (x_scale is not None):
         raise _lib.SpecVerifyError(-8, "x_scale goes with a float8_e4m3fn x, and only with it")
-    x2 = x if x.dim() == 2 else x.reshape(-1, k)
-    rows = x2.shape[0]
-    if x2.stride(1) != 1 or qweight.stride(1) != 1 or (groups > 1 and scales.stride(1) != 1):
+    if x.stride(-1) != 1 or qweight.stride(1) != 1 or (groups > 1 and scales.stride(1) != 1):
         raise _lib.SpecVerifyError(-3, "x, qweight and scales must have unit stride on their last dimension")
     if fp8 and (x_scale.dtype != torch.float32 or x_scale.shape != x.shape[:-1] or not x_scale.is_contiguous()):
         raise _lib.SpecVerifyError(-1, f"x_scale must be a contiguous float32 {list(x.shape[:-1])}")
-    if out is None:
-        res = torch.empty(x.shape[:-1] + (n,), dtype=scales.dtype, device=dev)
-        o_sm = n
-    else:
-        if out.shape != (rows, n) or out.dtype != scales.dtype or (n > 1 and out.stride(1) != 1) or (
-                rows > 1 and out.stride(0) < n):
-            raise _lib.SpecVerifyError(-1, f"out must be [{rows}, {n}] {scales.dtype} with unit column stride")
-        res, o_sm = out, out.stride(0)
-    a = _lib.W4Args()
-    a.out_dtype = _lib.TV_BF16 if scales.dtype == torch.bfloat16 else _lib.TV_F16
-    a.x_dtype = _lib.TV_E4M3 if fp8 else a.out_dtype
-    a.rows, a.n, a.k, a.group = rows, n, k, k // groups
-    a.x, a.x_sm = x2.data_ptr(), x2.stride(0)
-    a.x_scale = x_scale.data_ptr() if fp8 else None
-    a.qweight, a.q_sn = qweight.data_ptr(), qweight.stride(0) if n > 1 else k // 8
-    a.scales, a.s_sn = scales.data_ptr(), scales.stride(0)
-    a.out, a.o_sm = res.data_ptr(), o_sm
-    lib = _lib.load()
-    need = ctypes.c_size_t(0)
-    _lib.check(lib.tv_w4_workspace_size(ctypes.byref(a), ctypes.byref(need)), "tv_w4_workspace_size")
-    if need.value:
-        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), need.value
-    _lib.check(_lib.launch(dev, lib.tv_w4_linear, ctypes.byref(a)), "tv_w4_linear")
-    return res
+    rows = x.numel() // k
+    if out is not None and (out.shape != (rows, n) or out.dtype != scales.dtype or (n > 1 and out.stride(1) != 1)
+                            or (rows > 1 and out.stride(0) < n)):
+        raise _lib.SpecVerifyError(-1, f"out must be [{rows}, {n}] {scales.dtype} with unit column stride")
