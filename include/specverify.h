@@ -324,8 +324,10 @@ int tv_accept(const tv_accept_args* args, void* stream);
  * The walk goes on at the accepted child.  Where none is accepted the next
  * token is the first word at which the cumulated weight of what is left
  * exceeds uniform[0] * its sum (of p itself where nothing is left).
- * Sums and comparisons are in 64 bits; there are no atomics on values, so the
- * same inputs give the same result.
+ * Comparisons are in 64 bits, sums over the vocabulary in pairs of floats (a
+ * weight below 2^-126 of its row's largest counts as 0); there are no atomics
+ * on values, so the same inputs give the same result.  temperature from 1e-20
+ * to 1e20.
  *
  * parent / draft as tv_accept (parent -1: child of the root), and every parent
  * comes before its children.  counts (optional): sequence b has counts[b]

@@ -20,10 +20,20 @@
 // leaves a (max, sum) pair per chunk: bound by HBM.  Stage 2 (one cluster per
 // sequence) joins the pairs, walks the tree, and draws: the ending node's row
 // is split over the cluster's CTAs, whose sums meet through distributed
-// shared memory.  Whole numbers hang on comparisons here, so stage 2 computes
-// weights and sums in 64 bits; stage 1's normaliser (fp32 exponentials summed
-// in 64 bits) only enters the comparisons of a child's probability.
+// shared memory.
+//
+// Whole numbers hang on comparisons here.  A draw goes wrong when uniform[0]
+// falls between a border of the exact CDF and the computed one, and 128256
+// words have as many borders: with fp32 weights (2^-24 each) that is a few
+// draws in ten thousand.  Stage 2 therefore carries weights and sums as
+// unevaluated pairs of floats (about 2^-36 a weight, one draw in a million);
+// FP64 instructions would do too, but run at 1/24 of the fp32 rate here (49 us
+// for one row of 128256 words on eight SMs, against 4).  Stage 1's normaliser
+// (fp32 exponentials, summed in 64 bits) enters only the few comparisons of a
+// child's probability.
 #include <cooperative_groups.h>
+
+#include <cmath>
 
 #include "common.cuh"
 
@@ -43,11 +53,75 @@ template <> __device__ __forceinline__ float as_float<__nv_bfloat16>(__nv_bfloat
 template <> __device__ __forceinline__ float as_float<__half>(__half x) { return __half2float(x); }
 template <> __device__ __forceinline__ float as_float<float>(float x) { return x; }
 
-// Draft probabilities come in any of the three types, chosen at run time.
-__device__ __forceinline__ double load_prob(const void* p, int dtype, int64_t i) {
-  if (dtype == TV_F32) return (double)static_cast<const float*>(p)[i];
-  if (dtype == TV_F16) return (double)__half2float(static_cast<const __half*>(p)[i]);
-  return (double)__bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+// ---- pairs of floats: h + l, |l| at most half a step of h (Dekker; Knuth) -----
+struct Pair {
+  float h, l;
+};
+__device__ __forceinline__ Pair two_sum(float a, float b) {
+  const float s = a + b, bb = s - a;
+  return {s, (a - (s - bb)) + (b - bb)};
+}
+__device__ __forceinline__ Pair add(Pair a, Pair b) {
+  const Pair s = two_sum(a.h, b.h);
+  const float l = s.l + (a.l + b.l);
+  const float h = s.h + l;
+  return {h, l - (h - s.h)};
+}
+__device__ __forceinline__ double value(Pair a) { return (double)a.h + (double)a.l; }
+__device__ __forceinline__ Pair pair_of(double d) {
+  const float h = (float)d;
+  return {h, (float)(d - (double)h)};
+}
+__device__ __forceinline__ Pair warp_sum(Pair a) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    a = add(a, {__shfl_xor_sync(0xffffffffu, a.h, o), __shfl_xor_sync(0xffffffffu, a.l, o)});
+  return a;
+}
+
+constexpr int kTable = 1024;     // 2^(i / 1024) as pairs
+
+// Maximum that keeps a NaN of either side.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// How exponents become weights: 1024 log2(e) / T as a pair, and the smallest
+// l - m that is told from -inf (2^-200).
+struct Exponent {
+  Pair c;
+  float floor;
+};
+
+// exp((l - m) / T): t = (l - m) * 1024 log2(e) / T as a pair, its nearest
+// integer (by adding 1.5 * 2^23) splits into a power of two and a table entry,
+// and the rest r (at most 1/2) is 2^(r / 1024) = 1 + y + y^2 / 2 + y^3 / 6 with
+// y < 3.4e-4.  Below 2^-126 of the largest weight: 0.  The low part is up to
+// 3.4e-4 of the high one, no unevaluated rounding error, until it is summed.
+// l - m of 16-bit logits is exact or, for |l| below 2^-13 of m, off by 2^-24
+// of m at most; fp32 logits carry the difference's error along (EXACT).
+template <bool EXACT>
+__device__ __forceinline__ Pair weight_pair(float l, float m, const Exponent& c, const float2* table) {
+  float x, xl = 0.f;
+  if (EXACT) {
+    const Pair d = two_sum(l, -m);
+    x = max_nan(d.h, c.floor);
+    xl = x == d.h ? d.l : 0.f;
+  } else {
+    x = max_nan(l - m, c.floor);
+  }
+  const float t = x * c.c.h;
+  float tl = fmaf(x, c.c.l, fmaf(x, c.c.h, -t));
+  if (EXACT) tl = fmaf(xl, c.c.h, tl);
+  const float kf = t + 12582912.0f;
+  const float y = ((t - (kf - 12582912.0f)) + tl) * 6.7690154351557159e-4f;   // ln(2) / 1024
+  const int ki = __float_as_int(kf) - 0x4B400000;
+  const float2 e = table[ki & (kTable - 1)];
+  const float s = fmaf(y * y, fmaf(y, 1.0f / 6.0f, 0.5f), y);
+  const float scale = __int_as_float((max(ki >> 10, -127) + 127) << 23);
+  return {e.x * scale, fmaf(e.x, s, e.y) * scale};
 }
 
 struct Args {
@@ -63,30 +137,28 @@ struct Args {
   const float* uniform;
   int64_t u_sb;
   const void* probs;
-  int probs_dtype;
   int64_t q_sb, q_sm;
-  double inv_t;
-  float c_hi, c_lo;            // log2(e) / T as a sum of two floats
+  float c_hi, c_lo;            // log2(e) / T as a sum of two floats, c_lo > 0
+  Exponent exponent;
   float* part_max;             // [batch][rows][chunks]
   double* part_sum;
   int64_t* next_tokens;        // [batch][rows]
   int64_t* result;             // [batch][8 + 2 rows]
 };
 
-// exp((l - m) / T) in fp32: the product with log2(e) / T carries its rounding
-// error along, so the result is within a few 2^-23 at any magnitude.
+// exp((l - m) / T) in fp32.  Of the rounding errors only the product's own
+// stays, one of either sign a word; c_lo takes out that of log2(e) / T, which
+// all words share (and is positive, so that -inf stays -inf).
 __device__ __forceinline__ float weight32(float l, float m, float c_hi, float c_lo) {
   const float x = l - m;
-  const float t = x * c_hi;
-  const float r = fmaf(x, c_lo, fmaf(x, c_hi, -t));
-  const float e = fast_exp2(t);
-  return x == -INFINITY ? 0.f : fmaf(e, r * kLn2, e);
+  return fast_exp2(fmaf(x, c_lo, x * c_hi));
 }
 
 template <typename E>
 __global__ void __launch_bounds__(kStatThreads) row_stats_kernel(const Args a) {
   constexpr int VEC = 16 / sizeof(E);
   constexpr int U = kChunkBytes / (16 * kStatThreads);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int row = blockIdx.y, b = blockIdx.z;
   if (a.counts && row >= a.counts[b]) return;
   const int lo = blockIdx.x * a.chunk;
@@ -154,15 +226,16 @@ __global__ void __launch_bounds__(kStatThreads) row_stats_kernel(const Args a) {
 // so the draw finds its block without a second pass over the row.
 constexpr int kLane = 8;
 constexpr int kBlock = 32 * kLane;
-constexpr int kMarks = 64;              // 2048 marks of removed words, by word mod 2048
 
 struct Walk {
+  float2 table[kTable];
   double cta_sum[2][kMaxCluster];
-  uint32_t mark[kMarks];
   int status;
+  int removed;            // words taken out of the ending node's distribution, in dup[]
 };
 
-template <typename E>
+// Q: type of the draft probabilities (float without any when SAMPLED is false).
+template <typename E, typename Q, bool SAMPLED>
 __global__ void __launch_bounds__(kWalkThreads, 1) walk_kernel(const Args a) {
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), size = (int)cluster.num_blocks();
@@ -185,11 +258,15 @@ __global__ void __launch_bounds__(kWalkThreads, 1) walk_kernel(const Args a) {
   int64_t* result = a.result + (int64_t)b * (8 + 2 * rows);
   int64_t* next_tokens = a.next_tokens + (int64_t)b * rows;
   const E* logits = static_cast<const E*>(a.logits) + (int64_t)b * a.l_sb;
+  for (int i = tid; i < kTable; i += kWalkThreads) {
+    const Pair e = pair_of(exp2((double)i * (1.0 / kTable)));
+    sh.table[i] = make_float2(e.h, e.l);
+  }
   const int live = a.counts ? a.counts[b] : rows;
   const bool counted = live >= 1 && live <= rows;
   const int n = counted ? live : 0;
   if (tid == 0) sh.status = counted ? TV_OK : TV_ERR_INPUT;
-  if (tid < kMarks) sh.mark[tid] = 0;
+  if (tid == 0) sh.removed = 0;
   __syncthreads();
   // 1. the tree: every parent is an earlier node, every drafted token a word
   for (int i = tid; i < n; i += kWalkThreads) {
@@ -208,33 +285,64 @@ __global__ void __launch_bounds__(kWalkThreads, 1) walk_kernel(const Args a) {
     tok[i] = t;
     take[i] = -1;
   }
-  // 2. each node's maximum and normaliser from its chunks' pairs
-  for (int i = warp; i < n; i += kWalkWarps) {
-    const int64_t at = ((int64_t)b * rows + i) * a.chunks;
-    float m = -INFINITY;
-    for (int c = lane; c < a.chunks; c += 32) m = fmaxf(m, a.part_max[at + c]);
+  __syncthreads();
+  const bool bad = sh.status != TV_OK;
+  // the drafted words' logits and the draw's number, on their way while stage 1 ends
+  const float u0 = n > 0 ? u[0] : 0.f;
+  float child_logit[2];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float base = m == -INFINITY ? 0.f : m;
-    double s = 0.0;
-    for (int c = lane; c < a.chunks; c += 32)
-      s += a.part_sum[at + c] * exp(((double)a.part_max[at + c] - (double)base) * a.inv_t);
+  for (int q = 0; q < 2; ++q) {
+    const int i = tid + q * kWalkThreads;
+    child_logit[q] = i > 0 && i < n ? as_float<E>(logits[(int64_t)par[i] * a.l_sm + tok[i]]) : 0.f;
+  }
+  // 2. each node's maximum and normaliser from its chunks' pairs, four nodes'
+  // loads at a time
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int i0 = warp; i0 < n; i0 += 4 * kWalkWarps) {
+    float m[4], pm[4];
+    double ps[4], s[4];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) {
-      mx[i] = base;
-      z[i] = s;
+    for (int q = 0; q < 4; ++q) {
+      const int i = i0 + q * kWalkWarps;
+      const int64_t at = ((int64_t)b * rows + i) * a.chunks + lane;
+      const bool in = i < n && lane < a.chunks;
+      pm[q] = in ? a.part_max[at] : -INFINITY;
+      ps[q] = in ? a.part_sum[at] : 0.0;
+      m[q] = pm[q];
+      for (int c = 32; i < n && c + lane < a.chunks; c += 32) m[q] = fmaxf(m[q], a.part_max[at + c]);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m[q] = fmaxf(m[q], __shfl_xor_sync(0xffffffffu, m[q], o));
+      m[q] = m[q] == -INFINITY ? 0.f : m[q];
+      s[q] = ps[q] * (double)weight32(pm[q], m[q], a.c_hi, a.c_lo);
+      const int i = i0 + q * kWalkWarps;
+      const int64_t at = ((int64_t)b * rows + i) * a.chunks + lane;
+      for (int c = 32; i < n && c + lane < a.chunks; c += 32)
+        s[q] += a.part_sum[at + c] * (double)weight32(a.part_max[at + c], m[q], a.c_hi, a.c_lo);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) s[q] += __shfl_xor_sync(0xffffffffu, s[q], o);
+      const int i = i0 + q * kWalkWarps;
+      if (lane == 0 && i < n) {
+        mx[i] = m[q];
+        z[i] = s[q];
+      }
     }
   }
   __syncthreads();
-  const bool bad = sh.status != TV_OK;
-  for (int i = tid; i < n; i += kWalkThreads) {
-    if (i == 0) continue;
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int i = tid + q * kWalkThreads;
+    if (i < 1 || i >= n) continue;
     const int p = par[i];
-    const double l = (double)as_float<E>(logits[(int64_t)p * a.l_sm + tok[i]]);
-    prob[i] = exp((l - (double)mx[p]) * a.inv_t) / z[p];
+    prob[i] = value(weight_pair<true>(child_logit[q], mx[p], a.exponent, sh.table)) / z[p];
     int same = 0;
-    for (int j = p + 1; j < i; ++j) same |= par[j] == p && tok[j] == tok[i];
+#pragma unroll 8
+    for (int j = p + 1; j < i; ++j) same |= (par[j] == p) & (tok[j] == tok[i]);
     dup[i] = same;
   }
   cluster.sync();     // every CTA of the cluster runs before another writes to its shared memory
@@ -243,53 +351,105 @@ __global__ void __launch_bounds__(kWalkThreads, 1) walk_kernel(const Args a) {
   const int all_blocks = (vocab + kBlock - 1) / kBlock;
   const int my_blocks = max(0, min(a.blocks, all_blocks - first_block));
   int node = 0, length = 1;
-  double qa = 0.0, qb = 1.0, zq = 0.0;       // sampled drafts: (p - qa q)+, its sum; the row's exact normaliser
+  double qa = 0.0, qb = 1.0;                   // sampled drafts: (p - qa q)+ and its sum
   bool whole = false;                          // draw from p itself
   double left = 0.0;                           // sum of the weights that are drawn from
-  bool summed = false;
 
-  // What is left at the current node of the weights of words j0 + 32 k + lane.
-  auto weights = [&](int j0, double* w) {
+  Pair za = {0.f, 0.f}, aa = {0.f, 0.f};        // 1 / the row's sum of weights, and qa
+
+  // Logits (and draft probabilities) of words j0 + k * step of a block at the
+  // current node: none behind a branch of its own, so that all are in flight
+  // together.  Past the end of the vocabulary they are the last word's.
+  constexpr bool kExact = sizeof(E) == 4;
+  struct Words {
+    E l[kLane];
+    Q q[kLane];
+  };
+  auto load_words = [&](int j0, int step, Words& x) {
     const E* row = logits + (int64_t)node * a.l_sm;
-    const int64_t qoff = (int64_t)b * a.q_sb + (int64_t)node * a.q_sm;
-    const double base = (double)mx[node];
-    const bool minus = a.probs && qa > 0.0 && !whole;
-    float l[kLane];
-    double q[kLane];
+    const Q* qrow = static_cast<const Q*>(a.probs) + (int64_t)b * a.q_sb + (int64_t)node * a.q_sm;
+    if (j0 + kBlock <= vocab) {
 #pragma unroll
-    for (int k = 0; k < kLane; ++k) {
-      const int j = j0 + 32 * k + lane;
-      l[k] = j < vocab ? as_float<E>(row[j]) : -INFINITY;
-      q[k] = minus && j < vocab ? load_prob(a.probs, a.probs_dtype, qoff + j) : 0.0;
-    }
+      for (int k = 0; k < kLane; ++k) x.l[k] = row[j0 + step * k];
+      if (SAMPLED && qa > 0.0 && !whole) {
 #pragma unroll
-    for (int k = 0; k < kLane; ++k) {
-      const int j = j0 + 32 * k + lane;
-      double e = exp(((double)l[k] - base) * a.inv_t);
-      if (minus) {
-        const double d = e / zq - qa * q[k];
-        e = d < 0.0 ? 0.0 : d;
-      } else if (!a.probs && !whole && j < vocab && ((sh.mark[(j >> 5) & (kMarks - 1)] >> (j & 31)) & 1)) {
-        for (int i = node + 1; i < n; ++i)
-          if (par[i] == node && tok[i] == j && e == e) e = 0.0;
+        for (int k = 0; k < kLane; ++k) x.q[k] = qrow[j0 + step * k];
       }
-      w[k] = e;
+    } else {
+#pragma unroll
+      for (int k = 0; k < kLane; ++k) x.l[k] = row[min(j0 + step * k, vocab - 1)];
+      if (SAMPLED && qa > 0.0 && !whole) {
+#pragma unroll
+        for (int k = 0; k < kLane; ++k) x.q[k] = qrow[min(j0 + step * k, vocab - 1)];
+      }
     }
+  };
+  // What is left of their weights.
+  auto weigh = [&](int j0, int step, const Words& x, Pair* w) {
+    const float base = mx[node];
+#pragma unroll
+    for (int k = 0; k < kLane; ++k) w[k] = weight_pair<kExact>(as_float<E>(x.l[k]), base, a.exponent, sh.table);
+    if (SAMPLED && qa > 0.0 && !whole) {
+#pragma unroll
+      for (int k = 0; k < kLane; ++k) {
+        // p - qa q
+        const Pair e = w[k];
+        const float q = as_float<Q>(x.q[k]);
+        const float p = e.h * za.h;
+        const float pl = fmaf(e.h, za.l, fmaf(e.l, za.h, fmaf(e.h, za.h, -p)));
+        const float t = aa.h * q;
+        const float tl = fmaf(aa.l, q, fmaf(aa.h, q, -t));
+        const Pair d = two_sum(p, -t);
+        const float dl = d.l + (pl - tl), dh = d.h + dl;
+        w[k].h = dh < 0.f ? 0.f : dh;
+        w[k].l = dh < 0.f ? 0.f : dl - (dh - d.h);
+      }
+    }
+    if (!SAMPLED && !whole) {
+      // words taken out of the distribution: few, so first whether this block has any
+      const int lo = j0 - lane * (step == 1 ? kLane : 1);
+      bool any = false;
+      for (int i = lane; i < sh.removed; i += 32) any |= (unsigned)(dup[i] - lo) < (unsigned)kBlock;
+      if (__any_sync(0xffffffffu, any)) {
+        for (int i = 0; i < sh.removed; ++i)
+#pragma unroll
+          for (int k = 0; k < kLane; ++k)
+            if (dup[i] == j0 + step * k && w[k].l == w[k].l) w[k] = {0.f, 0.f};
+      }
+    }
+    if (j0 + kBlock > vocab) {
+#pragma unroll
+      for (int k = 0; k < kLane; ++k)
+        if (j0 + step * k >= vocab) w[k] = {0.f, 0.f};
+    }
+  };
+  // The eight words' sum, as a pair.
+  auto lane_sum = [&](const Pair* w) {
+    Pair s = w[0];
+#pragma unroll
+    for (int k = 1; k < kLane; ++k) {
+      const Pair t = two_sum(s.h, w[k].h);
+      s = {t.h, s.l + (t.l + w[k].l)};
+    }
+    const float h = s.h + s.l;
+    return Pair{h, s.l - (h - s.h)};
   };
   // Sum over the row: the blocks' sums stay in block_sum, the CTAs' in
   // sh.cta_sum[turn] of every CTA.  The two buffers alternate, so one cluster
-  // barrier a round is enough.
+  // barrier a round is enough.  A warp's next block is on its way while it
+  // sums the present one.
   int turn = 0;
   auto sum_row = [&] {
     __syncthreads();
+    Words next;
+    load_words((first_block + warp) * kBlock + lane, 32, next);
     for (int t = warp; t < my_blocks; t += kWalkWarps) {
-      double w[kLane], s = 0.0;
-      weights((first_block + t) * kBlock, w);
-#pragma unroll
-      for (int k = 0; k < kLane; ++k) s += w[k];
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (lane == 0) block_sum[t] = s;
+      const Words now = next;
+      load_words((first_block + t + kWalkWarps) * kBlock + lane, 32, next);
+      Pair w[kLane];
+      weigh((first_block + t) * kBlock + lane, 32, now, w);
+      const Pair s = warp_sum(lane_sum(w));
+      if (lane == 0) block_sum[t] = value(s);
     }
     __syncthreads();
     turn ^= 1;
@@ -302,19 +462,20 @@ __global__ void __launch_bounds__(kWalkThreads, 1) walk_kernel(const Args a) {
     }
     cluster.sync();
     double s = 0.0;
-    for (int r = 0; r < size; ++r) s += sh.cta_sum[turn][r];
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) s += r < size ? sh.cta_sum[turn][r] : 0.0;
     return s;
   };
 
   if (!bad) {
-    if (!a.probs) {
+    if constexpr (!SAMPLED) {
       // 3a. fixed drafts: every child is decided on its own
       for (int i = tid; i < n; i += kWalkThreads) {
         if (i == 0 || dup[i]) continue;
         const int p = par[i];
         double gone = 0.0;
-        for (int j = p + 1; j < i; ++j)
-          if (par[j] == p && !dup[j]) gone += prob[j];
+#pragma unroll 8
+        for (int j = p + 1; j < i; ++j) gone += par[j] == p && !dup[j] ? prob[j] : 0.0;
         if ((double)u[i] * (1.0 - gone) < prob[i]) atomicMin(reinterpret_cast<unsigned*>(&take[p]), (unsigned)i);
       }
       __syncthreads();
@@ -322,39 +483,62 @@ __global__ void __launch_bounds__(kWalkThreads, 1) walk_kernel(const Args a) {
         node = take[node];
         ++length;
       }
+      __syncthreads();              // dup is a list of words from here on
       for (int i = node + 1 + tid; i < n; i += kWalkThreads)
-        if (par[i] == node) atomicOr(&sh.mark[(tok[i] >> 5) & (kMarks - 1)], 1u << (tok[i] & 31));
-    } else {
-      // 3b. sampled drafts: node by node, each rejection a pass over the row
-      for (int i = 1; i < n; ++i) {
-        if (par[i] != node) continue;
-        const double q = load_prob(a.probs, a.probs_dtype, (int64_t)b * a.q_sb + (int64_t)node * a.q_sm + tok[i]);
-        const double d = prob[i] - (qa > 0.0 ? qa * q : 0.0);
-        if ((double)u[i] * qb * q < (d > 0.0 ? d : 0.0)) {
+        if (par[i] == node) dup[atomicAdd(&sh.removed, 1)] = (int)tok[i];
+    }
+    // 3b. sampled drafts: node by node, each rejection a pass over the row (the
+    // first one two: the row's own sum, then what is left).  4. The draw's
+    // pass, twice where nothing is left: then from the node's own
+    // distribution.  One loop, so that the pass's code is there once: run
+    // once or twice a launch, it costs as much to fetch as to execute.
+    enum { kScan, kRowSum, kRest, kDraw };
+    int want = SAMPLED ? kScan : kDraw, i = 1;
+    bool summed = false;
+    for (;;) {
+      if (SAMPLED && want == kScan) {
+        for (; i < n; ++i) {
+          if (par[i] != node) continue;
+          const Q* qrow = static_cast<const Q*>(a.probs) + (int64_t)b * a.q_sb + (int64_t)node * a.q_sm;
+          const double q = (double)as_float<Q>(qrow[tok[i]]);
+          const double d = prob[i] - (qa > 0.0 ? qa * q : 0.0);
+          if (!((double)u[i] * qb * q < (d > 0.0 ? d : 0.0))) break;
           if (tid == 0) take[node] = i;
           node = i;
           ++length;
           qa = 0.0;
           qb = 1.0;
           summed = false;
-        } else {
-          if (qa == 0.0) zq = sum_row();
+        }
+        if (i == n && summed && left != 0.0) break;
+        want = i == n ? kDraw : qa == 0.0 ? kRowSum : kRest;
+        if (want == kDraw) whole = summed;
+        if (want == kRest) {
           qa += qb;
-          left = qb = sum_row();
-          summed = true;
+          aa = pair_of(qa);
         }
       }
-    }
-    // 4. the draw: from the node's own distribution where nothing is left
-    if (!summed) left = sum_row();
-    if (left == 0.0) {
-      whole = true;
       left = sum_row();
+      if (SAMPLED && want == kRowSum) {
+        za = pair_of(1.0 / left);
+        qa = qb;
+        aa = pair_of(qa);
+        want = kRest;
+      } else if (SAMPLED && want == kRest) {
+        qb = left;
+        summed = true;
+        want = kScan;
+        ++i;
+      } else if (left == 0.0 && !whole) {
+        whole = true;
+      } else {
+        break;
+      }
     }
   }
   const bool fail = bad || !(left > 0.0) || left == (double)INFINITY;
   if (!fail) {
-    float uf = u[0];
+    float uf = u0;
     if (!(uf >= 0.f)) uf = 0.f;
     if (!(uf < 1.f)) uf = 0.99999994f;
     const double v = (double)uf * left;
@@ -400,25 +584,38 @@ __global__ void __launch_bounds__(kWalkThreads, 1) walk_kernel(const Args a) {
           run += __shfl_sync(0xffffffffu, c, 31);
         }
       }
-      double w[kLane];
-      const int j0 = (first_block + block) * kBlock;
-      weights(j0, w);
-      int pick = j0;
+      // eight consecutive words a lane: one scan over the lanes, then one lane's eight
+      Pair w[kLane];
+      Words x;
+      const int j0 = (first_block + block) * kBlock + lane * kLane;
+      load_words(j0, 1, x);
+      weigh(j0, 1, x, w);
+      int last = -1;                 // this lane's last word with any weight
+#pragma unroll
+      for (int k = 0; k < kLane; ++k)
+        if (w[k].h > 0.f) last = j0 + k;
+      const double mine = value(lane_sum(w));
+      double c = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double t = __shfl_up_sync(0xffffffffu, c, o);
+        if (lane >= o) c += t;
+      }
+      const unsigned over = __ballot_sync(0xffffffffu, last >= 0 && at + c > v);
+      const unsigned some = __ballot_sync(0xffffffffu, last >= 0);
+      const int at_lane = over ? __ffs(over) - 1 : 31 - __clz(some);
+      double run = at + (c - mine);
+      int pick = last;
       bool hit = false;
 #pragma unroll
       for (int k = 0; k < kLane; ++k) {
-        double c = w[k];
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double t = __shfl_up_sync(0xffffffffu, c, o);
-          if (lane >= o) c += t;
+        run += value(w[k]);
+        if (!hit && w[k].h > 0.f && run > v) {
+          pick = j0 + k;
+          hit = true;
         }
-        const unsigned over = __ballot_sync(0xffffffffu, w[k] > 0.0 && at + c > v);
-        const unsigned some = __ballot_sync(0xffffffffu, w[k] > 0.0);
-        if (!hit && some) pick = j0 + 32 * k + (over ? __ffs(over) - 1 : 31 - __clz(some));
-        hit |= over != 0;
-        at += __shfl_sync(0xffffffffu, c, 31);
       }
+      pick = __shfl_sync(0xffffffffu, pick, at_lane);
       if (lane == 0) {
         result[3] = pick;
         next_tokens[node] = pick;
@@ -451,36 +648,50 @@ __global__ void __launch_bounds__(kWalkThreads, 1) walk_kernel(const Args a) {
 int chunk_elems(int dtype) { return kChunkBytes / (dtype == TV_F32 ? 4 : 2); }
 int chunk_count(int dtype, int vocab) { return (vocab + chunk_elems(dtype) - 1) / chunk_elems(dtype); }
 
-// CTAs per sequence: one per 4096 words, up to the portable cluster size.
-int cluster_size(int vocab) {
-  int c = 1;
-  while (c < kMaxCluster && c * 4096 < vocab) c *= 2;
+// CTAs per sequence: one per 4096 words, as many as run at once (one per SM; as
+// the occupancy query reports it, clusters do not span processor groups).
+int cluster_size(int vocab, int batch) {
+  constexpr int fit[kMaxCluster + 1] = {0, 1 << 30, 74, 45, 33, 26, 22, 15, 15};
+  int c = kMaxCluster;
+  while (c > 1 && (batch > fit[c] || (c - 1) * 4096 >= vocab)) --c;
   return c;
 }
 
-template <typename E>
-int launch(const Args& a, int batch, size_t smem, cudaStream_t st) {
-  row_stats_kernel<E><<<dim3(a.chunks, a.rows, batch), kStatThreads, 0, st>>>(a);
-  int rc = check_launch();
-  if (rc != TV_OK) return rc;
-  if (smem > 40 * 1024) {
-    rc = ensure_dynamic_smem(reinterpret_cast<const void*>(walk_kernel<E>), (int)smem);
+template <typename E, typename Q, bool SAMPLED>
+int launch_walk(const Args& a, int batch, size_t smem, cudaStream_t st) {
+  if (smem > 32 * 1024) {
+    const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(walk_kernel<E, Q, SAMPLED>), (int)smem);
     if (rc != TV_OK) return rc;
   }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(cluster_size(a.vocab), batch);
+  const int size = cluster_size(a.vocab, batch);
+  cfg.gridDim = dim3(size, batch);
   cfg.blockDim = dim3(kWalkThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = cluster_size(a.vocab);
+  at[0].val.clusterDim.x = size;
   at[0].val.clusterDim.y = 1;
   at[0].val.clusterDim.z = 1;
+  // stage 2 starts while stage 1 ends and waits for its results on the device
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, walk_kernel<E>, a);
+  cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, walk_kernel<E, Q, SAMPLED>, a);
   return e == cudaSuccess ? check_launch() : record_cuda_error(e);
+}
+
+template <typename E>
+int launch(const Args& a, int probs_dtype, int batch, size_t smem, cudaStream_t st) {
+  row_stats_kernel<E><<<dim3(a.chunks, a.rows, batch), kStatThreads, 0, st>>>(a);
+  const int rc = check_launch();
+  if (rc != TV_OK) return rc;
+  if (!a.probs) return launch_walk<E, float, false>(a, batch, smem, st);
+  if (probs_dtype == TV_F32) return launch_walk<E, float, true>(a, batch, smem, st);
+  if (probs_dtype == TV_F16) return launch_walk<E, __half, true>(a, batch, smem, st);
+  return launch_walk<E, __nv_bfloat16, true>(a, batch, smem, st);
 }
 
 }  // namespace
@@ -504,7 +715,7 @@ int tv_residual_accept(const tv_residual_accept_args* a, void* stream) {
   if (a->rows > 1024 || a->batch > 65535 || a->vocab > (1 << 30)) return TV_ERR_UNSUPPORTED;
   if (a->logits_dtype < TV_BF16 || a->logits_dtype > TV_F32) return TV_ERR_DTYPE;
   if (a->probs && (a->probs_dtype < TV_BF16 || a->probs_dtype > TV_F32)) return TV_ERR_DTYPE;
-  if (!(a->temperature > 0.f) || !(a->temperature <= 3.4e38f)) return TV_ERR_INPUT;
+  if (!(a->temperature >= 1e-20f) || !(a->temperature <= 1e20f)) return TV_ERR_INPUT;   // log2(e) / T as a float
   if (a->batch == 0) return TV_OK;
   if (!a->logits || !a->draft || !a->uniform || !a->next_tokens || !a->result) return TV_ERR_NULL;
   if (a->rows > 1 && !a->parent) return TV_ERR_NULL;
@@ -528,27 +739,29 @@ int tv_residual_accept(const tv_residual_accept_args* a, void* stream) {
   k.uniform = a->uniform;
   k.u_sb = a->uniform_sb;
   k.probs = a->probs;
-  k.probs_dtype = a->probs_dtype;
   k.q_sb = a->probs_sb;
   k.q_sm = a->probs_sm;
-  k.inv_t = 1.0 / (double)a->temperature;
   const double c = 1.4426950408889634074 / (double)a->temperature;
   k.c_hi = (float)c;
+  while ((double)k.c_hi >= c) k.c_hi = nextafterf(k.c_hi, 0.f);
   k.c_lo = (float)(c - (double)k.c_hi);
+  k.exponent.c.h = (float)(1024.0 * c);
+  k.exponent.c.l = (float)(1024.0 * c - (double)k.exponent.c.h);
+  k.exponent.floor = (float)(-200.0 / c);
   k.part_sum = static_cast<double*>(a->workspace);
   k.part_max = reinterpret_cast<float*>(k.part_sum + (size_t)a->batch * a->rows * k.chunks);
   k.next_tokens = a->next_tokens;
   k.result = a->result;
-  const int words = cluster_size(a->vocab) * kBlock;
+  const int words = cluster_size(a->vocab, a->batch) * kBlock;
   k.blocks = (a->vocab + words - 1) / words;
   const size_t smem = (size_t)a->rows * (2 * sizeof(double) + sizeof(int64_t) + sizeof(float) + 3 * sizeof(int)) +
                       (size_t)k.blocks * sizeof(double);
   if (smem > 200 * 1024) return TV_ERR_UNSUPPORTED;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (a->logits_dtype) {
-    case TV_BF16: return launch<__nv_bfloat16>(k, a->batch, smem, st);
-    case TV_F16: return launch<__half>(k, a->batch, smem, st);
-    default: return launch<float>(k, a->batch, smem, st);
+    case TV_BF16: return launch<__nv_bfloat16>(k, a->probs_dtype, a->batch, smem, st);
+    case TV_F16: return launch<__half>(k, a->probs_dtype, a->batch, smem, st);
+    default: return launch<float>(k, a->probs_dtype, a->batch, smem, st);
   }
 }
 
