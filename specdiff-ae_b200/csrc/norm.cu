@@ -12,6 +12,8 @@
 // same pass and can hand the row on in 8 bits with its scale.
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "specverify.h"
 
@@ -154,55 +156,96 @@ struct AddNormArgs {
 
 // NC chunks per thread stay in registers; WIDE rows (more than that) are read
 // back from h, each thread its own chunks.
-template <typename T, bool FP8, int VEC, int NC, bool WIDE>
+//
+// SHIFT: rows that start off the 16-byte grid, x, r and h by the same offset
+// (dense tensors with an odd number of columns).  The chunks begin at the
+// row's first 16-byte boundary, the up to seven elements before and behind
+// them go one to a thread, and what lies otherwise (the weight; y unless its
+// offset is the same) is read or written element by element.
+template <typename T, bool FP8, int VEC, int NC, bool WIDE, bool SHIFT>
 __global__ void __launch_bounds__(512) add_rms_norm_kernel(const AddNormArgs a) {
   const T* x = static_cast<const T*>(a.x) + (int64_t)blockIdx.x * a.xs;
   const T* r = static_cast<const T*>(a.r) + (int64_t)blockIdx.x * a.rs;
   const T* w = static_cast<const T*>(a.w);
   T* h = static_cast<T*>(a.h) + (int64_t)blockIdx.x * a.hs;
+  T* y = static_cast<T*>(a.y) + (int64_t)blockIdx.x * a.ys;
+  uint8_t* y8 = static_cast<uint8_t*>(a.y) + (int64_t)blockIdx.x * a.ys;
+  const int head = SHIFT ? min(a.cols, (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T))) : 0;
+  const int end = SHIFT ? head + (a.cols - head) / VEC * VEC : a.cols;      // of the chunks
   const int step = blockDim.x * VEC;
-  const int first = threadIdx.x * VEC;
+  const int first = head + threadIdx.x * VEC;
+  // this thread's single element, if any
+  const int single = !SHIFT ? -1
+                     : (int)threadIdx.x < head ? (int)threadIdx.x
+                     : end + (int)threadIdx.x - head < a.cols ? end + (int)threadIdx.x - head : -1;
   Chunk<T, VEC> keep[NC];
+  Chunk<T, 1> one;
   float ss = 0.f;
+  // h = T(x + r), stored and squared
+  auto join = [&](auto& u, const auto& v, int c) {
+    constexpr int N = sizeof(u) / sizeof(T);
+    float f[N], g[N];
+    u.get(f);
+    v.get(g);
+#pragma unroll
+    for (int k = 0; k < N; ++k) f[k] += g[k];
+    u.set(f);
+    u.store(h + c);
+    u.get(f);
+#pragma unroll
+    for (int k = 0; k < N; ++k) ss = fmaf(f[k], f[k], ss);
+  };
   if (!WIDE) {
     Chunk<T, VEC> cr[NC];
+    Chunk<T, 1> cr1;
 #pragma unroll
     for (int i = 0; i < NC; ++i)
-      if (first + i * step < a.cols) {
+      if (first + i * step < end) {
         keep[i].load(x + first + i * step);
         cr[i].load(r + first + i * step);
       }
+    if (SHIFT && single >= 0) {
+      one.load(x + single);
+      cr1.load(r + single);
+    }
 #pragma unroll
     for (int i = 0; i < NC; ++i)
-      if (first + i * step < a.cols) {
-        float f[VEC], g[VEC];
-        keep[i].get(f);
-        cr[i].get(g);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) f[k] += g[k];
-        keep[i].set(f);
-        keep[i].store(h + first + i * step);
-        keep[i].get(f);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) ss = fmaf(f[k], f[k], ss);
-      }
+      if (first + i * step < end) join(keep[i], cr[i], first + i * step);
+    if (SHIFT && single >= 0) join(one, cr1, single);
   } else {
-    for (int c = first; c < a.cols; c += step) {
+    for (int c = first; c < end; c += step) {
       Chunk<T, VEC> u, v;
-      float f[VEC], g[VEC];
       u.load(x + c);
       v.load(r + c);
-      u.get(f);
-      v.get(g);
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) f[k] += g[k];
-      u.set(f);
-      u.store(h + c);
-      u.get(f);
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) ss = fmaf(f[k], f[k], ss);
+      join(u, v, c);
     }
   }
+  // What the thread holds of the row, chunk by chunk.
+  auto each = [&](auto&& fn) {
+    if (!WIDE) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        if (first + i * step < end) fn(keep[i], first + i * step);
+      if (SHIFT && single >= 0) fn(one, single);
+    } else {
+      for (int c = first; c < end; c += step) {
+        Chunk<T, VEC> u;
+        u.load(h + c);
+        fn(u, c);
+      }
+    }
+  };
+  auto weight = [&](int c, auto* g, auto n) {
+    constexpr int N = decltype(n)::value;
+    if constexpr (SHIFT && N > 1) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) g[k] = Elem<T>::to_f(w[c + k]);
+    } else {
+      Chunk<T, N> v;
+      v.load(w + c);
+      v.get(g);
+    }
+  };
   __shared__ float part[16];
   __shared__ float part_max[16];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
@@ -215,58 +258,33 @@ __global__ void __launch_bounds__(512) add_rms_norm_kernel(const AddNormArgs a) 
   const float inv = rsqrtf(tot / (float)a.cols + a.eps);
 
   if constexpr (!FP8) {
-    T* y = static_cast<T*>(a.y) + (int64_t)blockIdx.x * a.ys;
-    auto put = [&](const Chunk<T, VEC>& u, int c) {
-      Chunk<T, VEC> v;
-      float f[VEC], g[VEC];
-      v.load(w + c);
+    const bool whole = !SHIFT || ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(y)) & 15) == 0;
+    each([&](const auto& u, int c) {
+      constexpr int N = sizeof(u) / sizeof(T);
+      float f[N], g[N];
+      weight(c, g, std::integral_constant<int, N>{});
       u.get(f);
-      v.get(g);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) f[k] = round_to<T>(f[k] * inv) * g[k];
-      v.set(f);
-      v.store(y + c);
-    };
-    if (!WIDE) {
+      for (int k = 0; k < N; ++k) f[k] = round_to<T>(f[k] * inv) * g[k];
+      if (whole) {
+        Chunk<T, N> v;
+        v.set(f);
+        v.store(y + c);
+      } else {
 #pragma unroll
-      for (int i = 0; i < NC; ++i)
-        if (first + i * step < a.cols) put(keep[i], first + i * step);
-    } else {
-      for (int c = first; c < a.cols; c += step) {
-        Chunk<T, VEC> u;
-        u.load(h + c);
-        put(u, c);
+        for (int k = 0; k < N; ++k) y[c + k] = Elem<T>::from_f(f[k]);
       }
-    }
+    });
   } else {
-    uint8_t* y = static_cast<uint8_t*>(a.y) + (int64_t)blockIdx.x * a.ys;
-    auto row = [&](const Chunk<T, VEC>& u, int c, float* f) {
-      Chunk<T, VEC> v;
-      float g[VEC];
-      v.load(w + c);
-      u.get(f);
-      v.get(g);
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) f[k] = f[k] * inv * g[k];
-    };
     float mx = 0.f;
-    auto top = [&](const Chunk<T, VEC>& u, int c) {
-      float f[VEC];
-      row(u, c, f);
+    each([&](const auto& u, int c) {
+      constexpr int N = sizeof(u) / sizeof(T);
+      float f[N], g[N];
+      weight(c, g, std::integral_constant<int, N>{});
+      u.get(f);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) mx = max_nan(mx, fabsf(f[k]));
-    };
-    if (!WIDE) {
-#pragma unroll
-      for (int i = 0; i < NC; ++i)
-        if (first + i * step < a.cols) top(keep[i], first + i * step);
-    } else {
-      for (int c = first; c < a.cols; c += step) {
-        Chunk<T, VEC> u;
-        u.load(h + c);
-        top(u, c);
-      }
-    }
+      for (int k = 0; k < N; ++k) mx = max_nan(mx, fabsf(f[k] * inv * g[k]));
+    });
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     if (lane == 0) part_max[warp] = mx;
@@ -279,53 +297,61 @@ __global__ void __launch_bounds__(512) add_rms_norm_kernel(const AddNormArgs a) 
     // below 2^-100 is not safe to multiply with: divide there.
     const bool tiny = s < 7.8886091e-31f;
     const float is = 1.0f / s;
-    auto put = [&](const Chunk<T, VEC>& u, int c) {
-      float f[VEC];
-      row(u, c, f);
+    each([&](const auto& u, int c) {
+      constexpr int N = sizeof(u) / sizeof(T);
+      float f[N], g[N];
+      weight(c, g, std::integral_constant<int, N>{});
+      u.get(f);
       if (tiny) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) f[k] = s == 0.f ? 0.f : f[k] / s;
+        for (int k = 0; k < N; ++k) f[k] = s == 0.f ? 0.f : f[k] * inv * g[k] / s;
       } else {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) f[k] *= is;
+        for (int k = 0; k < N; ++k) f[k] = f[k] * inv * g[k] * is;
       }
-      store_e4m3<VEC>(y + c, f);
-    };
-    if (!WIDE) {
+      if constexpr (SHIFT && N > 1) {
 #pragma unroll
-      for (int i = 0; i < NC; ++i)
-        if (first + i * step < a.cols) put(keep[i], first + i * step);
-    } else {
-      for (int c = first; c < a.cols; c += step) {
-        Chunk<T, VEC> u;
-        u.load(h + c);
-        put(u, c);
+        for (int k = 0; k < N; ++k) store_e4m3<1>(y8 + c + k, f + k);
+      } else {
+        store_e4m3<N>(y8 + c, f);
       }
-    }
+    });
   }
 }
 
-template <typename T, bool FP8, int VEC, int NC, bool WIDE>
+template <typename T, bool FP8, int VEC, int NC, bool WIDE, bool SHIFT>
 int launch_add_norm(const AddNormArgs& a, int rows, int threads, cudaStream_t st) {
-  add_rms_norm_kernel<T, FP8, VEC, NC, WIDE><<<rows, threads, 0, st>>>(a);
+  add_rms_norm_kernel<T, FP8, VEC, NC, WIDE, SHIFT><<<rows, threads, 0, st>>>(a);
   return check_launch();
 }
 
-// Threads per row: enough that a row's chunks fit NC registers' worth, at most
-// 512 (a row of more than 512 * NC chunks is read back from h).
+enum AddNormLayout { kRowsAligned, kRowsShifted, kRowsAny };
+
+// Threads per row: as many as a row has chunks, at most 512; with enough rows
+// to fill the GPU, a quarter of them with four chunks each (NCM: fewer warps
+// meet at the reductions, and more rows are in flight per SM).  A row of more
+// than 2048 chunks is read back from h.
 template <typename T, bool FP8>
-int pick_add_norm(const AddNormArgs& a, int rows, bool vec, cudaStream_t st) {
-  const int chunks = vec ? a.cols / 8 : a.cols;
+int pick_add_norm(const AddNormArgs& a, int rows, AddNormLayout layout, cudaStream_t st) {
+  const int chunks = layout == kRowsAny ? a.cols : (a.cols + 7) / 8;
   auto fit = [&](int nc) { return ((chunks + nc - 1) / nc + 31) / 32 * 32; };
-  if (vec) {
-    if (fit(1) <= 512) return launch_add_norm<T, FP8, 8, 1, false>(a, rows, fit(1), st);
-    if (fit(2) <= 512) return launch_add_norm<T, FP8, 8, 2, false>(a, rows, fit(2), st);
-    if (fit(4) <= 512) return launch_add_norm<T, FP8, 8, 4, false>(a, rows, fit(4), st);
-    return launch_add_norm<T, FP8, 8, 1, true>(a, rows, 512, st);
+  const bool many = rows >= 8 * kNumSMs;
+  if (layout == kRowsAligned) {
+    if (fit(1) <= 512 && !(many && chunks >= 128)) return launch_add_norm<T, FP8, 8, 1, false, false>(a, rows, fit(1), st);
+    if (fit(2) <= 512 && !(many && chunks >= 256)) return launch_add_norm<T, FP8, 8, 2, false, false>(a, rows, fit(2), st);
+    if (fit(4) <= 512) return launch_add_norm<T, FP8, 8, 4, false, false>(a, rows, fit(4), st);
+    return launch_add_norm<T, FP8, 8, 1, true, false>(a, rows, 512, st);
   }
-  if (fit(4) <= 512) return launch_add_norm<T, FP8, 1, 4, false>(a, rows, fit(4), st);
-  if (fit(16) <= 512) return launch_add_norm<T, FP8, 1, 16, false>(a, rows, fit(16), st);
-  return launch_add_norm<T, FP8, 1, 1, true>(a, rows, 512, st);
+  if (layout == kRowsShifted) {
+    if (fit(1) <= 512 && !(many && chunks >= 128)) return launch_add_norm<T, FP8, 8, 1, false, true>(a, rows, fit(1), st);
+    if (fit(4) <= 512) return launch_add_norm<T, FP8, 8, 4, false, true>(a, rows, fit(4), st);
+  }
+  if (layout == kRowsAny || layout == kRowsShifted) {
+    const int t = (a.cols + 15) / 16 / 32 * 32 + 32;
+    if (a.cols <= 2048) return launch_add_norm<T, FP8, 1, 4, false, false>(a, rows, ((a.cols + 3) / 4 + 31) / 32 * 32, st);
+    if (t <= 512) return launch_add_norm<T, FP8, 1, 16, false, false>(a, rows, t, st);
+  }
+  return launch_add_norm<T, FP8, 1, 1, true, false>(a, rows, 512, st);
 }
 
 bool vec_ok(const void* p, int64_t stride) {
@@ -370,13 +396,24 @@ int tv_add_rms_norm(const void* x, int64_t x_row_stride, const void* residual, i
                 residual_out_row_stride, y_row_stride, cols, eps};
   const bool y_ok = y_scale ? (reinterpret_cast<uintptr_t>(y) & 7) == 0 && (y_row_stride % 8) == 0
                             : vec_ok(y, y_row_stride);
-  const bool vec = (cols % 8) == 0 && vec_ok(x, x_row_stride) && vec_ok(residual, residual_row_stride) &&
-                   vec_ok(weight, 0) && vec_ok(residual_out, residual_out_row_stride) && y_ok;
+  AddNormLayout layout = kRowsAny;
+  // one row needs no stride of its own
+  auto same = [&](const void* p, int64_t s) {
+    return ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(x)) & 15) == 0 &&
+           (rows == 1 || ((s - x_row_stride) & 7) == 0);
+  };
+  if ((cols % 8) == 0 && vec_ok(x, x_row_stride) && vec_ok(residual, residual_row_stride) && vec_ok(weight, 0) &&
+      vec_ok(residual_out, residual_out_row_stride) && y_ok)
+    layout = kRowsAligned;
+  else if (cols >= 64 && (reinterpret_cast<uintptr_t>(x) & 1) == 0 && same(residual, residual_row_stride) &&
+           same(residual_out, residual_out_row_stride))
+    layout = kRowsShifted;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == TV_BF16)
-    return y_scale ? pick_add_norm<__nv_bfloat16, true>(a, rows, vec, st)
-                   : pick_add_norm<__nv_bfloat16, false>(a, rows, vec, st);
-  return y_scale ? pick_add_norm<__half, true>(a, rows, vec, st) : pick_add_norm<__half, false>(a, rows, vec, st);
+    return y_scale ? pick_add_norm<__nv_bfloat16, true>(a, rows, layout, st)
+                   : pick_add_norm<__nv_bfloat16, false>(a, rows, layout, st);
+  return y_scale ? pick_add_norm<__half, true>(a, rows, layout, st)
+                 : pick_add_norm<__half, false>(a, rows, layout, st);
 }
 
 int tv_silu_mul(const void* gate, const void* up, int64_t in_row_stride, void* out, int64_t out_row_stride,
