@@ -329,8 +329,8 @@ int tv_accept(const tv_accept_args* args, void* stream);
  * on values, so the same inputs give the same result.  temperature from 1e-20
  * to 1e20.
  *
- * parent / draft as tv_accept (parent -1: child of the root), and every parent
- * comes before its children.  counts (optional): sequence b has counts[b]
+ * parent / draft as tv_accept (parent -1 or its own index: child of the root),
+ * and every parent comes before its children.  counts (optional): sequence b has counts[b]
  * nodes, 1 <= counts[b] <= rows; what lies behind them is not read.
  * result [batch][8 + 2 rows] as tv_accept's result, unused path entries -1;
  * next_tokens [batch][rows]: the drawn token at the last accepted node, -1

@@ -274,7 +274,8 @@ __global__ void __launch_bounds__(kWalkThreads, 1) walk_kernel(const Args a) {
     int p = 0;
     int64_t t = draft[i];
     if (i > 0) {
-      const int64_t pr = parent[i - 1];
+      int64_t pr = parent[i - 1];
+      if (pr == i - 1) pr = -1;
       if (pr < -1 || pr + 1 >= i || t < 0 || t >= vocab) {
         sh.status = TV_ERR_INPUT;
         t = 0;

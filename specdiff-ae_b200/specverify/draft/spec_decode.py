@@ -32,6 +32,14 @@ random-init weights, N(0, 0.02) as the reference's ``_init_weights``
 (``diffspec_model.py:100`` loads a tokenizer the decode loop never needs).
 With random weights acceptance is close to zero, so a step verifies about
 one token; the loop is a cost model of the real one, not a quality claim.
+
+``weight_bits=4`` holds the target's projections in 4 bits with group scales
+(``tv_w4_linear``); the residual's addition and the norm after it are then one
+launch (``tv_add_rms_norm``), with ``act_fp8`` handing the normalised rows to
+the next product in e4m3 with a scale per row.  ``acceptance="residual"``
+accepts by the residual rule (``tv_residual_accept``: the emitted tokens are
+the target's own distribution; the draft's tree is its top-k, so its drafts
+are fixed ones) instead of matching one sampled token per node.
 """
 
 from __future__ import annotations
@@ -44,10 +52,11 @@ from typing import Dict, List, Optional
 import torch
 
 from .. import _lib
+from ..runtime.lowbit import add_rms_norm, quantize_w4, w4_linear
 from ..runtime.rotary import rope_append
 from ..runtime.tree_attention import attention, pack_tree_mask
 from ..runtime.draft_tree import finalize_tree
-from .tree_verification import RESULT_HEADER, accept_from_hidden
+from .tree_verification import RESULT_HEADER, accept_from_hidden, accept_residual
 
 
 @dataclass
@@ -101,15 +110,17 @@ def rope_tables(head_dim: int, max_pos: int, theta: float, device, dtype=torch.b
 
 
 class _Layer:
-    """One decoder layer's weights (fused q/k/v and gate/up projections)."""
+    """One decoder layer's weights (fused q/k/v and gate/up projections); with
+    ``bits`` 4 a projection is the ``(qweight, scales)`` of :func:`quantize_w4`."""
 
-    def __init__(self, s: LlamaShape, in_dim: int, gen: torch.Generator, device, dtype):
+    def __init__(self, s: LlamaShape, in_dim: int, gen: torch.Generator, device, dtype, bits: int = 16,
+                 group: int = 128):
         qkv = s.heads * s.head_dim + 2 * s.kv_heads * s.head_dim
 
         def w(o, i):
             t = torch.empty(o, i, device=device, dtype=dtype)
             t.normal_(0.0, 0.02, generator=gen)
-            return t
+            return quantize_w4(t, group) if bits == 4 else t
         self.ln1 = torch.ones(in_dim, device=device, dtype=dtype)
         self.wqkv = w(qkv, in_dim)
         self.wo = w(s.hidden, s.heads * s.head_dim)
@@ -143,8 +154,13 @@ class SpecDecodeModel:
     """Target + EAGLE3-shaped draft head + paged caches, all on one GPU."""
 
     def __init__(self, shape: LlamaShape, device, dtype, gen: torch.Generator, max_tokens: int, draft_ctx: int,
-                 page_size: int = 16):
+                 page_size: int = 16, weight_bits: int = 16, group: int = 128, act_fp8: bool = False):
+        if weight_bits not in (4, 16):
+            raise ValueError(f"weight_bits {weight_bits} must be 4 or 16")
+        if act_fp8 and weight_bits != 4:
+            raise ValueError("act_fp8 needs weight_bits=4")
         s = self.shape = shape
+        self.weight_bits, self.act_fp8 = weight_bits, act_fp8
         self.device, self.dtype, self.page = device, dtype, page_size
         d = s.head_dim
 
@@ -153,7 +169,7 @@ class SpecDecodeModel:
             t.normal_(0.0, 0.02, generator=gen)
             return t
         self.embed = w(s.vocab, s.hidden)
-        self.layers = [_Layer(s, s.hidden, gen, device, dtype) for _ in range(s.layers)]
+        self.layers = [_Layer(s, s.hidden, gen, device, dtype, weight_bits, group) for _ in range(s.layers)]
         self.norm = torch.ones(s.hidden, device=device, dtype=dtype)
         self.lm_head = w(s.vocab, s.hidden)
         # draft head: fc over three target layers' hidden states, one layer
@@ -190,10 +206,13 @@ class SpecDecodeModel:
 
     @classmethod
     def from_config(cls, shape: Optional[LlamaShape] = None, *, device="cuda", dtype=torch.bfloat16, seed: int = 0,
-                    max_tokens: int = 65536 + 1024, draft_ctx: int = 2048) -> "SpecDecodeModel":
-        """Tokenizer-free constructor: random-init weights from ``seed``."""
+                    max_tokens: int = 65536 + 1024, draft_ctx: int = 2048, weight_bits: int = 16, group: int = 128,
+                    act_fp8: bool = False) -> "SpecDecodeModel":
+        """Tokenizer-free constructor: random-init weights from ``seed``
+        (the target's projections rounded to 4 bits with ``weight_bits=4``)."""
         gen = torch.Generator(device=device).manual_seed(seed)
-        return cls(shape or LlamaShape(), torch.device(device), dtype, gen, max_tokens, draft_ctx)
+        return cls(shape or LlamaShape(), torch.device(device), dtype, gen, max_tokens, draft_ctx,
+                   weight_bits=weight_bits, group=group, act_fp8=act_fp8)
 
     def fill_context(self, length: int, seed: int = 0):
         """Stand-in for the prefill of a ``length``-token prompt: the cache rows
@@ -211,6 +230,8 @@ class SpecDecodeModel:
         root-prepended mask bits [M, words]); returns the final normalised
         hidden [M, H] and the feature layers' hidden states [M, 3 H]."""
         s = self.shape
+        if self.weight_bits == 4:
+            return self._verify_w4(ids, pos, bits, start)
         x = self.embed[ids]
         feats = []
         for li, L in enumerate(self.layers):
@@ -219,6 +240,50 @@ class SpecDecodeModel:
             if li in s.feature_layers:
                 feats.append(x)
         return rms_norm(x, self.norm, s.rms_eps), torch.cat(feats, dim=-1)
+
+    def _verify_w4(self, ids: torch.Tensor, pos: torch.Tensor, bits: torch.Tensor, start: int):
+        """:meth:`verify` on 4-bit projections."""
+        s = self.shape
+        t = ids.numel()
+        vs = {"ids": ids, "pos": pos, "bits": bits, "x": torch.empty((t, s.hidden), dtype=self.dtype, device=self.device),
+              "qkv": torch.empty((t, (s.heads + 2 * s.kv_heads) * s.head_dim), dtype=self.dtype, device=self.device),
+              "qr": torch.empty((1, s.heads, t, s.head_dim), dtype=self.dtype, device=self.device),
+              "o": torch.empty((1, t, s.heads, s.head_dim), dtype=self.dtype, device=self.device),
+              "hidden": torch.empty((t, s.hidden), dtype=self.dtype, device=self.device),
+              "feats": torch.empty((t, len(s.feature_layers) * s.hidden), dtype=self.dtype, device=self.device)}
+        self._verify_segment_w4(vs, -1)
+        for li in range(s.layers):
+            self._verify_attend(vs, li, start, t)
+            self._verify_segment_w4(vs, li)
+        return vs["hidden"], vs["feats"]
+
+    def _verify_segment_w4(self, vs, li: int):
+        """:meth:`_verify_segment` on 4-bit projections: a product's output is
+        added to the residual stream by the norm that follows it."""
+        s = self.shape
+        x = vs["x"]
+
+        def add_norm(a, w):
+            """x += a and the normalised x, as the next product takes it."""
+            out = add_rms_norm(a, x, w, s.rms_eps, fp8=self.act_fp8, residual_out=x)
+            return (out[0], out[1]) if self.act_fp8 else (out[0], None)
+
+        if li < 0:
+            torch.index_select(self.embed, 0, vs["ids"], out=x)
+            L = self.layers[0]
+            w4_linear(rms_norm(x, L.ln1, s.rms_eps), *L.wqkv, out=vs["qkv"])
+            return
+        L = self.layers[li]
+        y, scale = add_norm(w4_linear(vs["o"].view(x.shape[0], -1), *L.wo), L.ln2)
+        down = w4_linear(silu_mul(w4_linear(y, *L.wgu, x_scale=scale), s.ffn), *L.wdown)
+        if li + 1 < s.layers:
+            y, scale = add_norm(down, self.layers[li + 1].ln1)
+            w4_linear(y, *self.layers[li + 1].wqkv, x_scale=scale, out=vs["qkv"])
+        else:
+            vs["hidden"].copy_(add_rms_norm(down, x, self.norm, s.rms_eps, residual_out=x)[0])
+        if li in s.feature_layers:
+            j = s.feature_layers.index(li)
+            vs["feats"][:, j * s.hidden:(j + 1) * s.hidden].copy_(x)
 
     def verify_graphed(self, ids: torch.Tensor, pos: torch.Tensor, bits: torch.Tensor, start: int):
         """:meth:`verify` with the torch work between two attention calls (the
@@ -246,6 +311,8 @@ class SpecDecodeModel:
     def _verify_segment(self, vs, li: int):
         """The torch work after layer li's attention (li = -1: the embedding)
         up to layer li + 1's q / k / v projection (or the final norm)."""
+        if self.weight_bits == 4:
+            return self._verify_segment_w4(vs, li)
         s = self.shape
         x = vs["x"]
         if li < 0:
@@ -361,9 +428,11 @@ class SpecDecodeModel:
 
     # ---- one speculative step ------------------------------------------------
     def step(self, root: torch.Tensor, root_feat: torch.Tensor, start: int, width: int, depth: int,
-             temperature: float, seed: int, offset: int, tree: Optional[Dict[str, torch.Tensor]] = None):
+             temperature: float, seed: int, offset: int, tree: Optional[Dict[str, torch.Tensor]] = None,
+             acceptance: str = "match"):
         """Draft (unless ``tree`` is given: a :func:`finalize_tree` result),
-        verify, accept, compact.  Returns (accept result, features of the tree
+        verify, accept (``acceptance`` "match" or, at a temperature, "residual"),
+        compact.  Returns (accept result, features of the tree
         rows [M, 3 H], CUDA events around the phases)."""
         ev = [torch.cuda.Event(enable_timing=True) for _ in range(4)]
         ev[0].record()
@@ -379,9 +448,14 @@ class SpecDecodeModel:
         else:
             hidden, feats = self.verify(ids, pos, tree["mask_bits"], start)
         ev[2].record()
-        acc = accept_from_hidden(hidden, self.lm_head, ids, parent, pos,
-                                 depth, mode="sample" if temperature > 0 else "greedy", temperature=temperature,
-                                 seed=seed, offset=offset)
+        if acceptance == "residual":
+            gen = torch.Generator(device=self.device).manual_seed((seed << 20) + offset)
+            uniform = torch.rand(ids.numel(), device=self.device, generator=gen)
+            acc = accept_residual(hidden @ self.lm_head.t(), ids, parent, uniform, temperature=temperature)
+        else:
+            acc = accept_from_hidden(hidden, self.lm_head, ids, parent, pos,
+                                     depth, mode="sample" if temperature > 0 else "greedy", temperature=temperature,
+                                     seed=seed, offset=offset)
         self._compact(start, acc, ids.numel())
         ev[3].record()
         return acc, feats, ev
@@ -426,9 +500,11 @@ class SpecDecodeModel:
 
     def diffspec_generate(self, prompt_len: int = 65536, max_new_tokens: int = 512, nodes: int = 64,
                           max_depth: int = 8, temperature: float = 1.0, seed: int = 0,
-                          max_steps: Optional[int] = None) -> Dict:
+                          max_steps: Optional[int] = None, acceptance: str = "match") -> Dict:
         """Decode ``max_new_tokens`` after a ``prompt_len``-token context (filled
-        by :meth:`fill_context`).  ``nodes`` = width x ``max_depth``.  One host
+        by :meth:`fill_context`).  ``acceptance``: "match" (the reference's rule:
+        a draft is accepted when the token sampled at its parent is the same) or
+        "residual" (speculative sampling's, needs a temperature).  ``nodes`` = width x ``max_depth``.  One host
         read per step (the accepted length, as the reference's loop reads it).
         Returns the tokens and per-phase device times."""
         width = nodes // max_depth
@@ -436,6 +512,10 @@ class SpecDecodeModel:
             raise ValueError("nodes must be a multiple of max_depth")
         if prompt_len + max_new_tokens + nodes + 2 > self.max_tokens:
             raise ValueError("cache too small for the request")
+        if acceptance not in ("match", "residual"):
+            raise ValueError(f"acceptance {acceptance!r} must be 'match' or 'residual'")
+        if acceptance == "residual" and not temperature > 0:
+            raise ValueError("the residual rule samples: it needs a temperature above 0")
         root_tok = self.fill_context(prompt_len, seed)
         root = torch.tensor([root_tok], device=self.device)
         root_feat = torch.zeros((1, 3 * self.shape.hidden), device=self.device, dtype=self.dtype)
@@ -448,10 +528,13 @@ class SpecDecodeModel:
         t0 = time.perf_counter()
         evs = []
         while len(out) < max_new_tokens and (max_steps is None or steps < max_steps):
-            acc, feats, ev = self.step(root, root_feat, start, width, max_depth, temperature, seed, offset=steps)
+            acc, feats, ev = self.step(root, root_feat, start, width, max_depth, temperature, seed, offset=steps,
+                                       acceptance=acceptance)
             evs.append(ev)
             res = acc.result
             n = int(res[2].item())                       # the one host read per step
+            if n < 1:
+                acc.to_host()                            # raises: the rule met a row that is no distribution
             toks = res[RESULT_HEADER + acc.rows:RESULT_HEADER + acc.rows + n].tolist()
             nxt = res[3:4]
             out.extend(toks[1:] + [None])                # accepted nodes, then the bonus token

@@ -191,8 +191,8 @@ def accept_residual(logits: torch.Tensor, draft: torch.Tensor, parent: torch.Ten
     token per node and matches the drafts against it instead.
 
     One tree: logits [M, V] (bf16, fp16 or fp32), draft [M] (the root first),
-    parent [M - 1] (-1: child of the root; a parent comes before its
-    children), uniform [M] fp32 in [0, 1): ``uniform[i]`` decides node i's
+    parent [M - 1] (-1 or the draft's own index: child of the root; a parent
+    comes before its children), uniform [M] fp32 in [0, 1): ``uniform[i]`` decides node i's
     draft, ``uniform[0]`` draws the final token.  A batch has a leading
     dimension everywhere; ``counts`` (int32 [B], or [1]) is then each
     sequence's number of nodes, the rest being padding that is not read.
@@ -219,7 +219,9 @@ def accept_residual(logits: torch.Tensor, draft: torch.Tensor, parent: torch.Ten
             and (m == 2 or parent.stride()[-1] == 1)
             and (draft_probs is None or (draft_probs.shape == shape and draft_probs.stride()[-1] == 1
                                          and draft_probs.dtype in _LOGITS and draft_probs.device == logits.device))
-            and counts is None and logits.device == draft.device == parent.device == uniform.device):
+            and (counts is None or (counts.shape == (b,) and counts.dtype is torch.int32 and counts.is_contiguous()
+                                    and counts.device == logits.device))
+            and logits.device == draft.device == parent.device == uniform.device):
         _check_accept_residual(logits, draft, parent, uniform, draft_probs, counts)
     code = _LOGITS[logits.dtype]
     nxt = draft.new_empty(own + (m,))

@@ -256,7 +256,7 @@ def test_bad_trees_are_reported_not_followed():
     lg = torch.randn(7, 4, 50, generator=g).cuda()
     draft = torch.randint(0, 50, (7, 4), generator=g)
     parent = torch.tensor([[-1, 0, 0]] * 7)
-    parent[1, 1] = 1                # itself
+    parent[1, 2] = 3                # past the tree
     parent[2, 1] = 2                # a later node
     parent[3, 0] = -2
     draft[4, 2] = 50
@@ -264,6 +264,10 @@ def test_bad_trees_are_reported_not_followed():
     counts = torch.tensor([4, 4, 4, 4, 4, 4, 5], dtype=torch.int32)
     acc = accept_residual(lg, draft.cuda(), parent.cuda(), torch.rand(7, 4, generator=g).cuda(), counts=counts.cuda())
     assert acc.result[:, 0].tolist() == [0] + [-6] * 6
+    # a draft's own index is another way to say "child of the root"
+    same = [accept_residual(lg[:1], draft[:1].cuda(), torch.tensor([p]).cuda(), torch.tensor([[0.5, 0.9, 0.9, 0.9]]).cuda())
+            for p in ([-1, -1, 1], [0, 1, 1])]
+    assert torch.equal(same[0].result, same[1].result) and same[0].result[0, 0].item() == 0
     counts[6] = 0
     acc = accept_residual(lg, draft.cuda(), parent.cuda(), torch.rand(7, 4, generator=g).cuda(), counts=counts.cuda())
     assert acc.result[6, 0].item() == -6 and acc.result[0, 0].item() == 0
