@@ -31,13 +31,14 @@
 #include <mutex>
 #include <type_traits>
 
-#include "common.cuh"
 #include "sm100.cuh"
+#include "w4.cuh"
 
 namespace tv {
 namespace {
 
 using namespace sm100;
+using namespace w4;
 namespace cg = cooperative_groups;
 
 constexpr int kRows = 128;                   // weight rows per CTA
@@ -76,54 +77,6 @@ struct W4Params {
   int split;                   // CTAs of a cluster
   uint32_t zero;               // 0, unknown to the compiler
   uint32_t group_magic;        // k / group = (k / 32) * magic >> 32; 0: group 32
-};
-
-template <typename T> __device__ __forceinline__ T bits_as(uint32_t u) { return *reinterpret_cast<T*>(&u); }
-template <typename T> __device__ __forceinline__ uint32_t as_bits(T v) { return *reinterpret_cast<uint32_t*>(&v); }
-
-// Eight packed weights -> four pairs of 16-bit values in k order.
-//
-// bf16: the bits 0 .. 255 read as a bf16 are that integer times 2^-133 (the
-// subnormal range and the first binade share a spacing), so a nibble masked at
-// bits 0-3 is u * 2^-133 and one at bits 4-7 is u * 2^-129, and ONE fused
-// multiply-add, (u * 2^-133) * (s * 2^(133 - 40)) - 8 s * 2^-40, gives
-// (u - 8) * s * 2^-40 rounded once: both factors and the addend are exact.
-// The accumulator is multiplied by 2^40 at the end.  Scales from 2^-80 to
-// 2^30 stay inside the exponent range.  9 instructions for 8 weights; the
-// usual 128 + u form needs a subtraction and a product, 15.
-//
-// fp16's exponents are too few for that: 1024 + u (or 1024 + 16 u), made by
-// OR, loses its offset in one exact operation, then the product rounds once.
-template <typename T> struct Unpack;
-template <> struct Unpack<__nv_bfloat16> {
-  __nv_bfloat162 sa, sb, off;
-  __device__ __forceinline__ void scale(uint32_t twice) {      // the scale's bits in both halves
-    const __nv_bfloat162 s2 = bits_as<__nv_bfloat162>(twice);
-    sa = __hmul2(s2, __float2bfloat162_rn(9.903520314283042e27f));      // 2^93
-    sb = __hmul2(s2, __float2bfloat162_rn(6.189700196426902e26f));      // 2^89
-    off = __hmul2(s2, __float2bfloat162_rn(-7.275957614183426e-12f));   // -2^-37
-  }
-  __device__ __forceinline__ void word(uint32_t w, uint32_t* o) const {
-    const uint32_t v = w >> 8;
-    o[0] = as_bits(__hfma2(bits_as<__nv_bfloat162>(w & 0x000F000Fu), sa, off));
-    o[1] = as_bits(__hfma2(bits_as<__nv_bfloat162>(w & 0x00F000F0u), sb, off));
-    o[2] = as_bits(__hfma2(bits_as<__nv_bfloat162>(v & 0x000F000Fu), sa, off));
-    o[3] = as_bits(__hfma2(bits_as<__nv_bfloat162>(v & 0x00F000F0u), sb, off));
-  }
-  static __device__ __forceinline__ float unscale() { return 1099511627776.0f; }   // 2^40
-};
-template <> struct Unpack<__half> {
-  __half2 s2;
-  __device__ __forceinline__ void scale(uint32_t twice) { s2 = bits_as<__half2>(twice); }
-  __device__ __forceinline__ void word(uint32_t w, uint32_t* o) const {
-    const uint32_t v = w >> 8;
-    const __half2 lo = __float2half2_rn(-1032.f), sixteenth = __float2half2_rn(0.0625f), hi = __float2half2_rn(-72.f);
-    o[0] = as_bits(__hmul2(__hadd2(bits_as<__half2>((w & 0x000F000Fu) | 0x64006400u), lo), s2));
-    o[1] = as_bits(__hmul2(__hfma2(bits_as<__half2>((w & 0x00F000F0u) | 0x64006400u), sixteenth, hi), s2));
-    o[2] = as_bits(__hmul2(__hadd2(bits_as<__half2>((v & 0x000F000Fu) | 0x64006400u), lo), s2));
-    o[3] = as_bits(__hmul2(__hfma2(bits_as<__half2>((v & 0x00F000F0u) | 0x64006400u), sixteenth, hi), s2));
-  }
-  static __device__ __forceinline__ float unscale() { return 1.0f; }
 };
 
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* v) {
@@ -409,22 +362,35 @@ __global__ void __launch_bounds__(kThreads, 2)
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
     if (warp >= kDequantWarp) {
-      int gave_up = 0;
-      for (int k = 0; k < p.split; ++k) gave_up |= *cluster.map_shared_rank(&bars->abort, k);
       const int tid = threadIdx.x - kDequantWarp * 32;
       const int r = tid & (kRows - 1);
       float* part = reinterpret_cast<float*>(smem);
       T* out = static_cast<T*>(p.out);
-      for (int j = rank + p.split * (tid / kRows); j < p.tokens; j += 2 * p.split) {
-        const int t = t0 + j;
-        if (t >= p.rows || n0 + r >= p.n) continue;
-        float v[kMaxCluster], f = 0.f;
+      int gave_up = 0;
 #pragma unroll
-        for (int k = 0; k < kMaxCluster; ++k) v[k] = k < p.split ? *cluster.map_shared_rank(part + j * kRows + r, k) : 0.f;
+      for (int k = 0; k < kMaxCluster; ++k) gave_up |= k < p.split ? *cluster.map_shared_rank(&bars->abort, k) : 0;
+      // this CTA's tokens, one of every p.split; three at a time, all of their
+      // parts on their way together
+      const int step = p.split * 2;
+#pragma unroll 1
+      for (int j0 = rank + p.split * (tid / kRows); j0 < p.tokens; j0 += 3 * step) {
+        float v[3][kMaxCluster];
 #pragma unroll
-        for (int k = 0; k < kMaxCluster; ++k) f += v[k];
-        if (gave_up) f = __int_as_float(0x7fc00000);
-        out[(int64_t)t * p.o_sm + n0 + r] = Elem<T>::from_f(p.x_scale ? f * p.x_scale[t] : f);
+        for (int i = 0; i < 3; ++i)
+#pragma unroll
+          for (int k = 0; k < kMaxCluster; ++k)
+            v[i][k] = k < p.split && j0 + i * step < p.tokens
+                          ? *cluster.map_shared_rank(part + (j0 + i * step) * kRows + r, k) : 0.f;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          const int j = j0 + i * step, t = t0 + j;
+          float f = 0.f;
+#pragma unroll
+          for (int k = 0; k < kMaxCluster; ++k) f += v[i][k];
+          if (gave_up) f = __int_as_float(0x7fc00000);
+          if (j < p.tokens && t < p.rows && n0 + r < p.n)
+            out[(int64_t)t * p.o_sm + n0 + r] = Elem<T>::from_f(p.x_scale ? f * p.x_scale[t] : f);
+        }
       }
     }
     cluster.sync();     // no CTA leaves while another still reads its sums
@@ -552,8 +518,7 @@ int launch_w4(const tv_w4_args* a, cudaStream_t st) {
   // rings: x tiles to cover an L2 round trip, the rest to the weights (3 to 5 stages)
   p.x_stages = p.tokens <= 16 ? 6 : p.tokens <= 48 ? 4 : p.tokens <= 80 ? 3 : 2;
   p.w_stages = (kRing - p.x_stages * p.x_bytes) / kWStage;
-  const uint32_t g32 = (uint32_t)a->group / 32;
-  p.group_magic = g32 == 1 ? 0 : (uint32_t)(((1ull << 32) + g32 - 1) / g32);
+  p.group_magic = group_magic(a->group);
   const int blocks_t = (a->rows + p.tokens - 1) / p.tokens;
   const int64_t tiles = (int64_t)((a->n + kRows - 1) / kRows) * blocks_t;
   const int stages = (a->k + kStageK - 1) / kStageK;
@@ -609,7 +574,7 @@ int tv_w4_workspace_size(const tv_w4_args* a, size_t* bytes) {
   if (!a || !bytes) return TV_ERR_NULL;
   const int rc = check_shape(a);
   if (rc != TV_OK) return rc;
-  *bytes = a->rows > 0 && staged(a) ? (size_t)a->rows * padded_k(a->k) * 2 : 0;
+  *bytes = a->rows > 0 && !w4_rows_fit(a) && staged(a) ? (size_t)a->rows * padded_k(a->k) * 2 : 0;
   return TV_OK;
 }
 
@@ -621,6 +586,7 @@ int tv_w4_linear(const tv_w4_args* a, void* stream) {
   if (!a->x || !a->qweight || !a->scales || !a->out || (a->x_dtype == TV_E4M3 && !a->x_scale)) return TV_ERR_NULL;
   if (!aligned16(a->qweight) || a->q_sn % 4 != 0) return TV_ERR_ALIGN;
   if (a->q_sn < a->k / 8) return TV_ERR_SHAPE;
+  if (w4_rows_fit(a)) return launch_w4_rows(a, static_cast<cudaStream_t>(stream));
   if (staged(a)) {
     size_t need = 0;
     tv_w4_workspace_size(a, &need);

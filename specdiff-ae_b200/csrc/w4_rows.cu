@@ -1,0 +1,300 @@
+// Up to 8 rows times 4-bit weights with group scales (one token, a draft's
+// frontier): the weights go from HBM through registers into mma.sync, with no
+// shared memory, tensor memory or barrier on their way.
+//
+// A team of 1, 2, 4 or 8 warps takes 16 weight rows at a time (M of m16n8k16;
+// the rows of x are its N) and splits k, 128 at a time: lane t of quad g loads
+// the 16 bytes, 32 weights, of k = 32 t .. 32 t + 31 of rows g and g + 8.
+// The MMA sums over k whatever its order, so the four lanes' k need not
+// interleave as the fragment's do, only match x's: x lies in shared memory
+// as 16-byte units of 8 k in the order ((128-k block, 8 k of 32), row, t), and a
+// B fragment of two MMAs is one conflict-free 16-byte load.  Four blocks' loads
+// are in flight per warp while the four before them are computed; the next 16
+// rows' follow on.  A team's sums meet in shared memory and are added in order.
+//
+// The loads alone take 13.0 us of the 18.7 at one row x 28672 x 4096 (9.0 at
+// the measured HBM rate): issue comes next to HBM, about 110 instructions a
+// warp for 2048 weights, 72 of them the unpacking.  The tcgen05 kernel has a
+// pipeline of five roles to start and drain and takes 21.4 there, 9.2 against
+// 5.2 at 4096 x 4096.
+#include <cuda_fp8.h>
+
+#include <type_traits>
+
+#include "w4.cuh"
+
+namespace tv {
+namespace {
+
+using namespace w4;
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kM = 16;                  // weight rows per unit
+constexpr int kBlockK = 128;
+constexpr int kBatch = 4;               // blocks in flight
+constexpr int kMaxRows = 8;             // N of m16n8k16; with two of them the tcgen05 kernel is the faster
+constexpr int kMaxSmem = 220 * 1024;
+
+struct Params {
+  const void* x;
+  int64_t x_sm;
+  const float* x_scale;
+  const uint32_t* q;
+  int64_t q_sn;
+  const void* s;
+  int64_t s_sn;
+  void* out;
+  int64_t o_sm;
+  int rows, n, k, blocks, units, split;
+  uint32_t magic;
+};
+
+// Eight consecutive values of a row as 16-bit pairs; zeros past k.
+template <typename X, typename T>
+__device__ __forceinline__ uint4 load8(const X* p, bool in, bool vec) {
+  uint4 o = make_uint4(0, 0, 0, 0);
+  if (!in) return o;
+  if constexpr (std::is_same<X, T>::value) {
+    if (vec) return *reinterpret_cast<const uint4*>(p);
+    uint32_t* w = reinterpret_cast<uint32_t*>(&o);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = (uint32_t) * reinterpret_cast<const uint16_t*>(p + 2 * i) |
+             (uint32_t) * reinterpret_cast<const uint16_t*>(p + 2 * i + 1) << 16;
+  } else {
+    X b[8];
+    if (vec) {
+      *reinterpret_cast<uint2*>(b) = *reinterpret_cast<const uint2*>(p);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) b[i] = p[i];
+    }
+    uint32_t* w = reinterpret_cast<uint32_t*>(&o);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = Elem<T>::pack2(static_cast<float>(b[2 * i]), static_cast<float>(b[2 * i + 1]));
+  }
+  return o;
+}
+
+// X: type of x (T or e4m3).  FOUR: group 128 with whole batches, the four
+// scales of one in one load.
+template <typename T, typename X, bool FOUR>
+__global__ void __launch_bounds__(kThreads, 2) w4_rows_kernel(const Params p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint4* xs = reinterpret_cast<uint4*>(smem);
+  float* red = reinterpret_cast<float*>(smem + (size_t)p.blocks * kBlockK * 2 * p.rows);   // [2][warps][8][16]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  // split warps share 16 weight rows, each its run of 128-k blocks
+  const int part = warp % p.split, team = warp / p.split, teams = kWarps / p.split;
+  const int lo = p.blocks * part / p.split, hi = p.blocks * (part + 1) / p.split;
+  const int stride = gridDim.x * teams;
+
+  struct Batch {
+    uint4 w[kBatch][2];
+    uint32_t s[kBatch][2];      // a block's scales; with FOUR [0][h], [1][h] are the batch's four
+  };
+  // Blocks b .. b + 3 of rows 16 unit + g and + 8; rows past the end repeat the
+  // last one (not stored), k past the end weighs nothing.
+  const bool even = p.k % kBlockK == 0;
+  auto load = [&](int unit, int b, Batch& o) {
+    const int64_t n0 = min(unit * kM + g, p.n - 1), n1 = min(unit * kM + g + 8, p.n - 1);
+    const uint32_t* q0 = p.q + n0 * p.q_sn + (b * (kBlockK / 8) + t * 4);
+    const uint32_t* q1 = p.q + n1 * p.q_sn + (b * (kBlockK / 8) + t * 4);
+    const T* s0 = static_cast<const T*>(p.s) + n0 * p.s_sn;
+    const T* s1 = static_cast<const T*>(p.s) + n1 * p.s_sn;
+    auto words4 = [](const uint32_t* at, uint4& v) {
+      asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(at));
+    };
+    auto scale1 = [](const T* at, uint32_t& v) {
+      asm volatile("{\n\t.reg .u16 v;\n\tld.global.nc.u16 v, [%1];\n\tcvt.u32.u16 %0, v;\n\t}" : "=r"(v) : "l"(at));
+    };
+    auto index = [&](int i) {
+      const uint32_t u = (uint32_t)((b + i) * 4 + t);
+      return p.magic ? __umulhi(u, p.magic) : u;
+    };
+    if (FOUR) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        words4(q0 + i * (kBlockK / 8), o.w[i][0]);
+        words4(q1 + i * (kBlockK / 8), o.w[i][1]);
+      }
+      asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(o.s[0][0]), "=r"(o.s[1][0]) : "l"(s0 + b));
+      asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(o.s[0][1]), "=r"(o.s[1][1]) : "l"(s1 + b));
+    } else if (even && b + kBatch <= hi) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        words4(q0 + i * (kBlockK / 8), o.w[i][0]);
+        words4(q1 + i * (kBlockK / 8), o.w[i][1]);
+        const uint32_t j = index(i);
+        scale1(s0 + j, o.s[i][0]);
+        scale1(s1 + j, o.s[i][1]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        o.w[i][0] = o.w[i][1] = make_uint4(0, 0, 0, 0);
+        o.s[i][0] = o.s[i][1] = 0;
+        if (b + i < hi && ((b + i) * 4 + t) * 32 < p.k) {
+          words4(q0 + i * (kBlockK / 8), o.w[i][0]);
+          words4(q1 + i * (kBlockK / 8), o.w[i][1]);
+          const uint32_t j = index(i);
+          scale1(s0 + j, o.s[i][0]);
+          scale1(s1 + j, o.s[i][1]);
+        }
+      }
+    }
+  };
+  Batch ping, pong;
+  int unit = blockIdx.x * teams + team, b = lo;
+  if (unit < p.units) load(unit, b, ping);
+
+  // x into shared memory while the first weights are on their way
+  {
+    const X* x = static_cast<const X*>(p.x);
+    const int chunks = p.blocks * (kBlockK / 8);
+    const int total = p.rows * chunks;
+    const bool vec = (reinterpret_cast<uintptr_t>(x) % (8 * sizeof(X))) == 0 && (p.rows == 1 || p.x_sm % 8 == 0);
+    // unit e of the layout: 8 k of (block and 8 of 32, row, t)
+#pragma unroll 4
+    for (int e = threadIdx.x; e < total; e += kThreads) {
+      const int kj = (e >> 2) / p.rows, r = (e >> 2) - kj * p.rows;
+      const int c = (kj >> 2) * 16 + (e & 3) * 4 + (kj & 3);     // its k is 8 c
+      xs[e] = load8<X, T>(x + (int64_t)r * p.x_sm + c * 8, c * 8 < p.k, vec);
+    }
+  }
+  __syncthreads();
+
+  // this lane's row of x (column of B) in xs; past the last row, whose sums
+  // are not stored, the last
+  const int xrow = min(g, p.rows - 1) * 4;
+  int turn = 0;
+  float acc[4] = {};
+  auto put = [&](int r, int n, float sum) {
+    sum *= Unpack<T>::unscale();
+    if (p.x_scale) sum *= __ldg(p.x_scale + r);
+    static_cast<T*>(p.out)[(int64_t)r * p.o_sm + n] = Elem<T>::from_f(sum);
+  };
+  // One batch of the present unit, the one after it on its way; at the unit's
+  // end the warps' sums.  False once there is no unit left.
+  auto step = [&](const Batch& now, Batch& next) {
+    const bool last = b + kBatch >= hi;
+    if (!last) load(unit, b + kBatch, next);
+    else if (unit + stride < p.units) load(unit + stride, lo, next);
+    const uint4* xb = xs + b * 16 * p.rows + t;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (!FOUR && b + i >= hi) break;
+      Unpack<T> u0, u1;
+      u0.scale(FOUR ? __byte_perm(now.s[i >> 1][0], 0, i & 1 ? 0x3232 : 0x1010) : now.s[i][0] * 0x10001u);
+      u1.scale(FOUR ? __byte_perm(now.s[i >> 1][1], 0, i & 1 ? 0x3232 : 0x1010) : now.s[i][1] * 0x10001u);
+      const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&now.w[i][0]);
+      const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&now.w[i][1]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t a0[4], a1[4];
+        u0.word(w0[j], a0);
+        u1.word(w1[j], a1);
+        const uint32_t f0[4] = {a0[0], a1[0], a0[1], a1[1]}, f1[4] = {a0[2], a1[2], a0[3], a1[3]};
+        const uint4 v = xb[(i * 4 + j) * p.rows * 4 + xrow];
+        Mma<T>::run(acc, f0, v.x, v.y);
+        Mma<T>::run(acc, f1, v.z, v.w);
+      }
+    }
+    b += kBatch;
+    if (!last) return true;
+    // accumulator i of a lane: weight row g + 8 (i / 2), x row 2 t + i % 2
+    if (p.split == 1) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 2 * t + (i & 1), n = unit * kM + g + 8 * (i >> 1);
+        if (r < p.rows && n < p.n) put(r, n, acc[i]);
+        acc[i] = 0.f;
+      }
+    } else {
+      float* mine = red + (turn * kWarps + warp) * (kM * kMaxRows);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        mine[(2 * t + (i & 1)) * kM + g + 8 * (i >> 1)] = acc[i];
+        acc[i] = 0.f;
+      }
+      asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(p.split * 32) : "memory");
+      const float* ours = red + (turn * kWarps + team * p.split) * (kM * kMaxRows);
+      for (int e = part * 32 + lane; e < kM * p.rows; e += p.split * 32) {
+        const int n = unit * kM + e % kM;
+        float v[kWarps], sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) v[w] = w < p.split ? ours[w * (kM * kMaxRows) + e] : 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) sum += v[w];
+        if (n < p.n) put(e / kM, n, sum);
+      }
+    }
+    turn ^= 1;      // the other half is free: every warp of the team has passed the barrier after reading it
+    b = lo;
+    unit += stride;
+    return unit < p.units;
+  };
+  if (unit < p.units)
+    while (step(ping, pong) && step(pong, ping)) {
+    }
+}
+
+size_t smem_bytes(const tv_w4_args* a) {
+  const size_t blocks = (a->k + kBlockK - 1) / kBlockK;
+  return blocks * kBlockK * 2 * a->rows + 2 * kWarps * kM * kMaxRows * sizeof(float);
+}
+
+template <typename T, typename X, bool FOUR>
+int start(const Params& p, int grid, size_t smem, cudaStream_t st) {
+  const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(w4_rows_kernel<T, X, FOUR>), (int)smem);
+  if (rc != TV_OK) return rc;
+  w4_rows_kernel<T, X, FOUR><<<grid, kThreads, smem, st>>>(p);
+  return check_launch();
+}
+
+template <typename T, typename X>
+int launch(const tv_w4_args* a, Params p, size_t smem, cudaStream_t st) {
+  const int slots = kNumSMs * (smem <= 112 * 1024 ? 2 : 1);
+  // teams of as many warps as it takes to busy three quarters of those that fit
+  p.split = 1;
+  while (p.split < kWarps && 4 * p.units * p.split < 3 * slots * kWarps && p.blocks >= p.split * 2) p.split *= 2;
+  const int ctas = (p.units * p.split + kWarps - 1) / kWarps;
+  const int grid = ctas < slots ? ctas : slots;
+  const bool four = a->group == kBlockK && p.blocks % (p.split * kBatch) == 0 && a->s_sn % 4 == 0 &&
+                    reinterpret_cast<uintptr_t>(a->scales) % 8 == 0;
+  return four ? start<T, X, true>(p, grid, smem, st) : start<T, X, false>(p, grid, smem, st);
+}
+
+template <typename T>
+int dispatch(const tv_w4_args* a, const Params& p, size_t smem, cudaStream_t st) {
+  return a->x_dtype == TV_E4M3 ? launch<T, __nv_fp8_e4m3>(a, p, smem, st) : launch<T, T>(a, p, smem, st);
+}
+
+}  // namespace
+
+bool w4_rows_fit(const tv_w4_args* a) { return a->rows <= kMaxRows && smem_bytes(a) <= kMaxSmem; }
+
+int launch_w4_rows(const tv_w4_args* a, cudaStream_t st) {
+  Params p{};
+  p.x = a->x;
+  p.x_sm = a->x_sm;
+  p.x_scale = a->x_dtype == TV_E4M3 ? a->x_scale : nullptr;
+  p.q = static_cast<const uint32_t*>(a->qweight);
+  p.q_sn = a->q_sn;
+  p.s = a->scales;
+  p.s_sn = a->s_sn;
+  p.out = a->out;
+  p.o_sm = a->o_sm;
+  p.rows = a->rows;
+  p.n = a->n;
+  p.k = a->k;
+  p.blocks = (a->k + kBlockK - 1) / kBlockK;
+  p.units = (a->n + kM - 1) / kM;
+  p.magic = group_magic(a->group);
+  const size_t smem = smem_bytes(a);
+  return a->out_dtype == TV_BF16 ? dispatch<__nv_bfloat16>(a, p, smem, st) : dispatch<__half>(a, p, smem, st);
+}
+
+}  // namespace tv
