@@ -2,21 +2,27 @@
 // frontier): the weights go from HBM through registers into mma.sync, with no
 // shared memory, tensor memory or barrier on their way.
 //
-// A team of 1, 2, 4 or 8 warps takes 16 weight rows at a time (M of m16n8k16;
-// the rows of x are its N) and splits k, 128 at a time: lane t of quad g loads
-// the 16 bytes, 32 weights, of k = 32 t .. 32 t + 31 of rows g and g + 8.
-// The MMA sums over k whatever its order, so the four lanes' k need not
-// interleave as the fragment's do, only match x's: x lies in shared memory
-// as 16-byte units of 8 k in the order ((128-k block, 8 k of 32), row, t), and a
-// B fragment of two MMAs is one conflict-free 16-byte load.  Four blocks' loads
-// are in flight per warp while the four before them are computed; the next 16
-// rows' follow on.  A team's sums meet in shared memory and are added in order.
+// One CTA per SM, so that x is staged once an SM; its four teams of four warps
+// take 16 weight rows at a time (M of m16n8k16; the rows of x are its N),
+// dealt out SM by SM so that none has more than one unit above another.  A
+// team's warps split k, 128 at a time: lane t of quad g loads the 16 bytes, 32
+// weights, of k = 32 t .. 32 t + 31 of rows g and g + 8.  The MMA sums over k
+// whatever its order, so the four lanes' k need not interleave as the
+// fragment's do, only match x's: x lies in shared memory as 16-byte units of
+// 8 k in the order ((128-k block, 8 k of 32), row, t), and a B fragment of two
+// MMAs is one conflict-free 16-byte load.  Eight blocks of 128 k are in flight
+// per warp: each block's registers are loaded anew, eight blocks ahead, as soon
+// as it is used.  A team's sums meet in shared memory and are added in order.
 //
-// The loads alone take 13.0 us of the 18.7 at one row x 28672 x 4096 (9.0 at
-// the measured HBM rate): issue comes next to HBM, about 110 instructions a
-// warp for 2048 weights, 72 of them the unpacking.  The tcgen05 kernel has a
-// pipeline of five roles to start and drain and takes 21.4 there, 9.2 against
-// 5.2 at 4096 x 4096.
+// One row x 28672 x 4096 takes 17.2 us, 8 rows 18.6 (9.0 at the measured HBM
+// rate; the loads alone 13.0): issue comes next to HBM, about 140 instructions
+// a warp for 2048 weights, 72 of them the unpacking.  Two CTAs of eight warps
+// an SM, up to 16 units on one SM and 8 on another, took 18.8 and 21.9; one
+// batch of four blocks in flight instead of two 18.5 and 20.3 at teams of four.
+// Whole units a warp (no split of k) run 18.9 at 8 x 28672 x 4096, but 10.4 for
+// 7.7 at 8 x 6144 x 4096; teams of eight 19.5 and 8.1.  The tcgen05 kernel has a
+// pipeline of five roles to start and drain: 21.4 at one row x 28672 x 4096, 9.2
+// against 4.8 at 4096 x 4096.
 #include <cuda_fp8.h>
 
 #include <type_traits>
@@ -28,8 +34,10 @@ namespace {
 
 using namespace w4;
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
+constexpr int kTeam = 4;                // warps that share 16 weight rows
+constexpr int kTeams = kWarps / kTeam;
 constexpr int kM = 16;                  // weight rows per unit
 constexpr int kBlockK = 128;
 constexpr int kBatch = 4;               // blocks in flight
@@ -46,7 +54,7 @@ struct Params {
   int64_t s_sn;
   void* out;
   int64_t o_sm;
-  int rows, n, k, blocks, units, split;
+  int rows, n, k, blocks, units;
   uint32_t magic;
 };
 
@@ -63,7 +71,7 @@ __device__ __forceinline__ uint4 load8(const X* p, bool in, bool vec) {
       w[i] = (uint32_t) * reinterpret_cast<const uint16_t*>(p + 2 * i) |
              (uint32_t) * reinterpret_cast<const uint16_t*>(p + 2 * i + 1) << 16;
   } else {
-    X b[8];
+    alignas(8) X b[8];
     if (vec) {
       *reinterpret_cast<uint2*>(b) = *reinterpret_cast<const uint2*>(p);
     } else {
@@ -80,75 +88,80 @@ __device__ __forceinline__ uint4 load8(const X* p, bool in, bool vec) {
 // X: type of x (T or e4m3).  FOUR: group 128 with whole batches, the four
 // scales of one in one load.
 template <typename T, typename X, bool FOUR>
-__global__ void __launch_bounds__(kThreads, 2) w4_rows_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const Params p) {
   extern __shared__ __align__(16) uint8_t smem[];
   uint4* xs = reinterpret_cast<uint4*>(smem);
   float* red = reinterpret_cast<float*>(smem + (size_t)p.blocks * kBlockK * 2 * p.rows);   // [2][warps][8][16]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  // split warps share 16 weight rows, each its run of 128-k blocks
-  const int part = warp % p.split, team = warp / p.split, teams = kWarps / p.split;
-  const int lo = p.blocks * part / p.split, hi = p.blocks * (part + 1) / p.split;
-  const int stride = gridDim.x * teams;
+  // a warp's run of 128-k blocks, none where there are fewer than warps
+  const int part = warp % kTeam, team = warp / kTeam;
+  const int lo = p.blocks * part / kTeam, hi = p.blocks * (part + 1) / kTeam;
+  const int stride = gridDim.x * kTeams;
 
   struct Batch {
     uint4 w[kBatch][2];
     uint32_t s[kBatch][2];      // a block's scales; with FOUR [0][h], [1][h] are the batch's four
   };
-  // Blocks b .. b + 3 of rows 16 unit + g and + 8; rows past the end repeat the
-  // last one (not stored), k past the end weighs nothing.
-  const bool even = p.k % kBlockK == 0;
-  auto load = [&](int unit, int b, Batch& o) {
-    const int64_t n0 = min(unit * kM + g, p.n - 1), n1 = min(unit * kM + g + 8, p.n - 1);
-    const uint32_t* q0 = p.q + n0 * p.q_sn + (b * (kBlockK / 8) + t * 4);
-    const uint32_t* q1 = p.q + n1 * p.q_sn + (b * (kBlockK / 8) + t * 4);
-    const T* s0 = static_cast<const T*>(p.s) + n0 * p.s_sn;
-    const T* s1 = static_cast<const T*>(p.s) + n1 * p.s_sn;
-    auto words4 = [](const uint32_t* at, uint4& v) {
-      asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(at));
-    };
-    auto scale1 = [](const T* at, uint32_t& v) {
-      asm volatile("{\n\t.reg .u16 v;\n\tld.global.nc.u16 v, [%1];\n\tcvt.u32.u16 %0, v;\n\t}" : "=r"(v) : "l"(at));
-    };
-    auto index = [&](int i) {
-      const uint32_t u = (uint32_t)((b + i) * 4 + t);
-      return p.magic ? __umulhi(u, p.magic) : u;
-    };
-    if (FOUR) {
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        words4(q0 + i * (kBlockK / 8), o.w[i][0]);
-        words4(q1 + i * (kBlockK / 8), o.w[i][1]);
-      }
-      asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(o.s[0][0]), "=r"(o.s[1][0]) : "l"(s0 + b));
-      asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(o.s[0][1]), "=r"(o.s[1][1]) : "l"(s1 + b));
-    } else if (even && b + kBatch <= hi) {
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        words4(q0 + i * (kBlockK / 8), o.w[i][0]);
-        words4(q1 + i * (kBlockK / 8), o.w[i][1]);
-        const uint32_t j = index(i);
-        scale1(s0 + j, o.s[i][0]);
-        scale1(s1 + j, o.s[i][1]);
+  // What is loaded next: block b of unit's rows 16 unit + g and + 8; rows past
+  // the end repeat the last one (not stored), k past the end weighs nothing.
+  struct Ahead {
+    int unit, b;
+    const uint32_t *q0, *q1;
+    const T *s0, *s1;
+  } ahead{(int)(blockIdx.x + gridDim.x * team), lo, nullptr, nullptr, nullptr, nullptr};
+  auto at_unit = [&] {
+    const int64_t n0 = min(ahead.unit * kM + g, p.n - 1), n1 = min(ahead.unit * kM + g + 8, p.n - 1);
+    ahead.q0 = p.q + n0 * p.q_sn + t * 4;
+    ahead.q1 = p.q + n1 * p.q_sn + t * 4;
+    ahead.s0 = static_cast<const T*>(p.s) + n0 * p.s_sn;
+    ahead.s1 = static_cast<const T*>(p.s) + n1 * p.s_sn;
+  };
+  auto words4 = [](const uint32_t* at, uint4& v) {
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(at));
+  };
+  auto scale1 = [](const T* at, uint32_t& v) {
+    asm volatile("{\n\t.reg .u16 v;\n\tld.global.nc.u16 v, [%1];\n\tcvt.u32.u16 %0, v;\n\t}" : "=r"(v) : "l"(at));
+  };
+  auto load_block = [&](int i, Batch& o) {
+    const int b = ahead.b + i;
+    if (FOUR || (b < hi && (b * 4 + t) * 32 < p.k)) {
+      words4(ahead.q0 + b * (kBlockK / 8), o.w[i][0]);
+      words4(ahead.q1 + b * (kBlockK / 8), o.w[i][1]);
+      if (!FOUR) {
+        const uint32_t u = (uint32_t)(b * 4 + t), j = p.magic ? __umulhi(u, p.magic) : u;
+        scale1(ahead.s0 + j, o.s[i][0]);
+        scale1(ahead.s1 + j, o.s[i][1]);
       }
     } else {
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        o.w[i][0] = o.w[i][1] = make_uint4(0, 0, 0, 0);
-        o.s[i][0] = o.s[i][1] = 0;
-        if (b + i < hi && ((b + i) * 4 + t) * 32 < p.k) {
-          words4(q0 + i * (kBlockK / 8), o.w[i][0]);
-          words4(q1 + i * (kBlockK / 8), o.w[i][1]);
-          const uint32_t j = index(i);
-          scale1(s0 + j, o.s[i][0]);
-          scale1(s1 + j, o.s[i][1]);
-        }
-      }
+      o.s[i][0] = o.s[i][1] = 0;
     }
   };
-  Batch ping, pong;
-  int unit = blockIdx.x * teams + team, b = lo;
-  if (unit < p.units) load(unit, b, ping);
+  auto load_four = [&](Batch& o) {
+    asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(o.s[0][0]), "=r"(o.s[1][0]) : "l"(ahead.s0 + ahead.b));
+    asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(o.s[0][1]), "=r"(o.s[1][1]) : "l"(ahead.s1 + ahead.b));
+  };
+  auto advance = [&] {
+    ahead.b += kBatch;
+    if (ahead.b >= hi) {
+      ahead.b = lo;
+      ahead.unit += stride;
+      at_unit();
+    }
+  };
+  Batch ping{}, pong{};
+  int unit = ahead.unit, b = lo;
+  at_unit();
+  auto fill = [&](Batch& o) {
+    if (ahead.unit < p.units) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) load_block(i, o);
+      if (FOUR) load_four(o);
+      advance();
+    }
+  };
+  fill(ping);
+  fill(pong);
 
   // x into shared memory while the first weights are on their way
   {
@@ -171,65 +184,57 @@ __global__ void __launch_bounds__(kThreads, 2) w4_rows_kernel(const Params p) {
   const int xrow = min(g, p.rows - 1) * 4;
   int turn = 0;
   float acc[4] = {};
-  auto put = [&](int r, int n, float sum) {
-    sum *= Unpack<T>::unscale();
-    if (p.x_scale) sum *= __ldg(p.x_scale + r);
-    static_cast<T*>(p.out)[(int64_t)r * p.o_sm + n] = Elem<T>::from_f(sum);
-  };
-  // One batch of the present unit, the one after it on its way; at the unit's
-  // end the warps' sums.  False once there is no unit left.
-  auto step = [&](const Batch& now, Batch& next) {
-    const bool last = b + kBatch >= hi;
-    if (!last) load(unit, b + kBatch, next);
-    else if (unit + stride < p.units) load(unit + stride, lo, next);
+  // One batch of the present unit, each block's registers refilled two batches
+  // ahead as soon as it is used; at the unit's end the warps' sums.  False once
+  // there is no unit left.
+  auto step = [&](Batch& now) {
+    const bool last = b + kBatch >= hi, more = ahead.unit < p.units;
     const uint4* xb = xs + b * 16 * p.rows + t;
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      if (!FOUR && b + i >= hi) break;
-      Unpack<T> u0, u1;
-      u0.scale(FOUR ? __byte_perm(now.s[i >> 1][0], 0, i & 1 ? 0x3232 : 0x1010) : now.s[i][0] * 0x10001u);
-      u1.scale(FOUR ? __byte_perm(now.s[i >> 1][1], 0, i & 1 ? 0x3232 : 0x1010) : now.s[i][1] * 0x10001u);
-      const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&now.w[i][0]);
-      const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&now.w[i][1]);
+      if (FOUR || b + i < hi) {
+        Unpack<T> u0, u1;
+        u0.scale(FOUR ? __byte_perm(now.s[i >> 1][0], 0, i & 1 ? 0x3232 : 0x1010) : now.s[i][0] * 0x10001u);
+        u1.scale(FOUR ? __byte_perm(now.s[i >> 1][1], 0, i & 1 ? 0x3232 : 0x1010) : now.s[i][1] * 0x10001u);
+        const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&now.w[i][0]);
+        const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&now.w[i][1]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t a0[4], a1[4];
-        u0.word(w0[j], a0);
-        u1.word(w1[j], a1);
-        const uint32_t f0[4] = {a0[0], a1[0], a0[1], a1[1]}, f1[4] = {a0[2], a1[2], a0[3], a1[3]};
-        const uint4 v = xb[(i * 4 + j) * p.rows * 4 + xrow];
-        Mma<T>::run(acc, f0, v.x, v.y);
-        Mma<T>::run(acc, f1, v.z, v.w);
+        for (int j = 0; j < 4; ++j) {
+          uint32_t a0[4], a1[4];
+          u0.word(w0[j], a0);
+          u1.word(w1[j], a1);
+          const uint32_t f0[4] = {a0[0], a1[0], a0[1], a1[1]}, f1[4] = {a0[2], a1[2], a0[3], a1[3]};
+          const uint4 v = xb[(i * 4 + j) * p.rows * 4 + xrow];
+          Mma<T>::run(acc, f0, v.x, v.y);
+          Mma<T>::run(acc, f1, v.z, v.w);
+        }
       }
+      if (more) load_block(i, now);
+    }
+    if (more) {
+      if (FOUR) load_four(now);
+      advance();
     }
     b += kBatch;
     if (!last) return true;
     // accumulator i of a lane: weight row g + 8 (i / 2), x row 2 t + i % 2
-    if (p.split == 1) {
+    float* mine = red + (turn * kWarps + warp) * (kM * kMaxRows);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 2 * t + (i & 1), n = unit * kM + g + 8 * (i >> 1);
-        if (r < p.rows && n < p.n) put(r, n, acc[i]);
-        acc[i] = 0.f;
-      }
-    } else {
-      float* mine = red + (turn * kWarps + warp) * (kM * kMaxRows);
+    for (int i = 0; i < 4; ++i) {
+      mine[(2 * t + (i & 1)) * kM + g + 8 * (i >> 1)] = acc[i];
+      acc[i] = 0.f;
+    }
+    asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(kTeam * 32) : "memory");
+    const float* ours = red + (turn * kWarps + team * kTeam) * (kM * kMaxRows);
+    const int e = part * 32 + lane, n = unit * kM + e % kM;
+    static_assert(kTeam * 32 == kM * kMaxRows, "a thread of the team per sum");
+    if (e / kM < p.rows && n < p.n) {
+      float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        mine[(2 * t + (i & 1)) * kM + g + 8 * (i >> 1)] = acc[i];
-        acc[i] = 0.f;
-      }
-      asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(p.split * 32) : "memory");
-      const float* ours = red + (turn * kWarps + team * p.split) * (kM * kMaxRows);
-      for (int e = part * 32 + lane; e < kM * p.rows; e += p.split * 32) {
-        const int n = unit * kM + e % kM;
-        float v[kWarps], sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) v[w] = w < p.split ? ours[w * (kM * kMaxRows) + e] : 0.f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) sum += v[w];
-        if (n < p.n) put(e / kM, n, sum);
-      }
+      for (int w = 0; w < kTeam; ++w) sum += ours[w * (kM * kMaxRows) + e];
+      sum *= Unpack<T>::unscale();
+      if (p.x_scale) sum *= __ldg(p.x_scale + e / kM);
+      static_cast<T*>(p.out)[(int64_t)(e / kM) * p.o_sm + n] = Elem<T>::from_f(sum);
     }
     turn ^= 1;      // the other half is free: every warp of the team has passed the barrier after reading it
     b = lo;
@@ -237,7 +242,7 @@ __global__ void __launch_bounds__(kThreads, 2) w4_rows_kernel(const Params p) {
     return unit < p.units;
   };
   if (unit < p.units)
-    while (step(ping, pong) && step(pong, ping)) {
+    while (step(ping) && step(pong)) {
     }
 }
 
@@ -256,13 +261,8 @@ int start(const Params& p, int grid, size_t smem, cudaStream_t st) {
 
 template <typename T, typename X>
 int launch(const tv_w4_args* a, Params p, size_t smem, cudaStream_t st) {
-  const int slots = kNumSMs * (smem <= 112 * 1024 ? 2 : 1);
-  // teams of as many warps as it takes to busy three quarters of those that fit
-  p.split = 1;
-  while (p.split < kWarps && 4 * p.units * p.split < 3 * slots * kWarps && p.blocks >= p.split * 2) p.split *= 2;
-  const int ctas = (p.units * p.split + kWarps - 1) / kWarps;
-  const int grid = ctas < slots ? ctas : slots;
-  const bool four = a->group == kBlockK && p.blocks % (p.split * kBatch) == 0 && a->s_sn % 4 == 0 &&
+  const int grid = p.units < kNumSMs ? p.units : kNumSMs;
+  const bool four = a->group == kBlockK && p.blocks % (kTeam * kBatch) == 0 && a->s_sn % 4 == 0 &&
                     reinterpret_cast<uintptr_t>(a->scales) % 8 == 0;
   return four ? start<T, X, true>(p, grid, smem, st) : start<T, X, false>(p, grid, smem, st);
 }
