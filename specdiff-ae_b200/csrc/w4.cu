@@ -338,22 +338,31 @@ __global__ void __launch_bounds__(kThreads, 2)
     tc_fence_after();
     T* out = static_cast<T*>(p.out);
     float* part = reinterpret_cast<float*>(smem);        // [token][weight row], once both rings are drained
+    const bool in = n0 + r < p.n;
 #pragma unroll 1
     for (int c = g; c * 16 < p.tokens; c += 2) {
       uint32_t v[16];
       tmem_ld16(lanes + (uint32_t)(c * 16), v);
       tmem_wait_ld();
-      const int t = t0 + c * 16;
+      const int t = t0 + c * 16, left = in ? p.rows - t : 0;
+      float f[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) f[j] = ok ? __uint_as_float(v[j]) * Unpack<T>::unscale() : __int_as_float(0x7fc00000);
+      // no branch per token: each costs what a store does
+      if (p.split > 1) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) part[(c * 16 + j) * kRows + r] = f[j];
+        continue;
+      }
+      if (p.x_scale) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) f[j] *= __ldg(p.x_scale + min(t + j, p.rows - 1));
+      }
       T* at = out + (int64_t)t * p.o_sm + n0 + r;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        float f = ok ? __uint_as_float(v[j]) * Unpack<T>::unscale() : __int_as_float(0x7fc00000);
-        if (p.split > 1) {
-          part[(c * 16 + j) * kRows + r] = f;
-        } else if (t + j < p.rows && n0 + r < p.n) {
-          if (p.x_scale) f *= __ldg(p.x_scale + t + j);
-          at[j * p.o_sm] = Elem<T>::from_f(f);
-        }
+        if (j < left) *at = Elem<T>::from_f(f[j]);
+        at += p.o_sm;
       }
     }
   }
