@@ -20,9 +20,18 @@
 // CTAs splits k; the partial sums meet in distributed shared memory and are
 // added in rank order, so results do not depend on timing.
 //
-// Bound by HBM (the packed weights once) up to about 80 tokens, by the tensor
-// pipe above.  Each (u - 8) * s is rounded once to x's 16-bit type (the MMA
-// takes no other): half a step, as the weight itself had in that type.
+// Each (u - 8) * s is rounded once to x's 16-bit type (the MMA takes no other):
+// half a step, as the weight itself had in that type.
+//
+// What bounds it: an MMA of 128 rows x 16 k takes about 37 cycles however few
+// the tokens (its A operand's way out of tensor memory), so a stage is 0.32 us of
+// an SM's tensor pipe, and two CTAs there were seen to take 0.37 a stage: 65
+// rows x 28672 x 4096 spend 12 of 23.5 us in that (16 stages, two CTAs on half of
+// the SMs, one on the others), 3.3 until the first weights are there and 4 from
+// the last MMA to the end.  128 rows x 128256 x 4096: 119 us, 1.13 PFLOP/s.
+// Tiles of 256 weight rows with k cut evenly over the SMs balance better and were
+// slower, as were pairs of CTAs splitting k (37 us): partial sums cost more
+// than idle SMs.  Weights as the B operand would pad the tokens to 128.
 #include <cooperative_groups.h>
 #include <cuda.h>
 #include <cuda_fp8.h>
@@ -85,6 +94,20 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* v) {
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
         "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
       : "r"(taddr));
+}
+
+// The address of a shared-memory word in another CTA of the cluster, and a load
+// from there; 0 where `in` is false.
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, int rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr, bool in) {
+  float v;
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.f32 %0, 0f00000000;\n\t@p ld.shared::cluster.f32 %0, [%1];\n\t}"
+               : "=f"(v) : "r"(addr), "r"((uint32_t)in) : "memory");
+  return v;
 }
 
 // Loads in flight land before shared memory is reused or released: a producer
@@ -373,13 +396,12 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (warp >= kDequantWarp) {
       const int tid = threadIdx.x - kDequantWarp * 32;
       const int r = tid & (kRows - 1);
-      float* part = reinterpret_cast<float*>(smem);
       T* out = static_cast<T*>(p.out);
-      int gave_up = 0;
+      uint32_t part[kMaxCluster];            // this row's sums in every CTA
 #pragma unroll
-      for (int k = 0; k < kMaxCluster; ++k) gave_up |= k < p.split ? *cluster.map_shared_rank(&bars->abort, k) : 0;
+      for (int k = 0; k < kMaxCluster; ++k) part[k] = map_rank(smem_u32(smem) + r * 4, min(k, p.split - 1));
       // this CTA's tokens, one of every p.split; three at a time, all of their
-      // parts on their way together
+      // parts on their way together.  A CTA that gave up left NaNs.
       const int step = p.split * 2;
 #pragma unroll 1
       for (int j0 = rank + p.split * (tid / kRows); j0 < p.tokens; j0 += 3 * step) {
@@ -388,17 +410,15 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (int i = 0; i < 3; ++i)
 #pragma unroll
           for (int k = 0; k < kMaxCluster; ++k)
-            v[i][k] = k < p.split && j0 + i * step < p.tokens
-                          ? *cluster.map_shared_rank(part + (j0 + i * step) * kRows + r, k) : 0.f;
+            v[i][k] = ld_cluster(part[k] + (j0 + i * step) * (kRows * 4), k < p.split && j0 + i * step < p.tokens);
 #pragma unroll
         for (int i = 0; i < 3; ++i) {
           const int j = j0 + i * step, t = t0 + j;
           float f = 0.f;
 #pragma unroll
           for (int k = 0; k < kMaxCluster; ++k) f += v[i][k];
-          if (gave_up) f = __int_as_float(0x7fc00000);
-          if (j < p.tokens && t < p.rows && n0 + r < p.n)
-            out[(int64_t)t * p.o_sm + n0 + r] = Elem<T>::from_f(p.x_scale ? f * p.x_scale[t] : f);
+          if (p.x_scale) f *= __ldg(p.x_scale + min(t, p.rows - 1));
+          if (j < p.tokens && t < p.rows && n0 + r < p.n) out[(int64_t)t * p.o_sm + n0 + r] = Elem<T>::from_f(f);
         }
       }
     }
