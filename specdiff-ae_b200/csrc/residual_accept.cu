@@ -297,14 +297,15 @@ __global__ void __launch_bounds__(kWalkThreads, 1) walk_kernel(const Args a) {
     const int i = tid + q * kWalkThreads;
     child_logit[q] = i > 0 && i < n ? as_float<E>(logits[(int64_t)par[i] * a.l_sm + tok[i]]) : 0.f;
   }
-  // 2. each node's maximum and normaliser from its chunks' pairs, four nodes'
-  // loads at a time
+  // 2. each node's maximum and normaliser from its chunks' pairs, five nodes'
+  // loads at a time (a tree of 64 and its root in one turn)
+  constexpr int kNodes = 5;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  for (int i0 = warp; i0 < n; i0 += 4 * kWalkWarps) {
-    float m[4], pm[4];
-    double ps[4], s[4];
+  for (int i0 = warp; i0 < n; i0 += kNodes * kWalkWarps) {
+    float m[kNodes], pm[kNodes];
+    double ps[kNodes], s[kNodes];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < kNodes; ++q) {
       const int i = i0 + q * kWalkWarps;
       const int64_t at = ((int64_t)b * rows + i) * a.chunks + lane;
       const bool in = i < n && lane < a.chunks;
@@ -314,7 +315,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) walk_kernel(const Args a) {
       for (int c = 32; i < n && c + lane < a.chunks; c += 32) m[q] = fmaxf(m[q], a.part_max[at + c]);
     }
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < kNodes; ++q) {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m[q] = fmaxf(m[q], __shfl_xor_sync(0xffffffffu, m[q], o));
       m[q] = m[q] == -INFINITY ? 0.f : m[q];
@@ -325,7 +326,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) walk_kernel(const Args a) {
         s[q] += a.part_sum[at + c] * (double)weight32(a.part_max[at + c], m[q], a.c_hi, a.c_lo);
     }
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < kNodes; ++q) {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) s[q] += __shfl_xor_sync(0xffffffffu, s[q], o);
       const int i = i0 + q * kWalkWarps;

@@ -17,6 +17,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libspecverify.so"
 
 TV_OK = 0
 TV_BF16, TV_F16, TV_F32, TV_E4M3 = 0, 1, 2, 3
+TV_ERR_WORKSPACE = -5
 
 _DTYPE_CODE = {torch.bfloat16: TV_BF16, torch.float16: TV_F16, torch.float32: TV_F32}
 

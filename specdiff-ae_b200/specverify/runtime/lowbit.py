@@ -3,6 +3,8 @@
 * :func:`add_rms_norm` -- the residual's addition and ``LlamaRMSNorm``
   (``runtime/llama_target_model.py:124-138``) in one pass, with a 16-bit output
   or an e4m3 one with a scale per row.
+* :func:`w4_linear` -- the projections of such a layer with 4-bit weights and
+  group scales, laid out by :func:`quantize_w4`.
 
 CUDA tensors only; errors raise :class:`specverify.SpecVerifyError`.
 """
@@ -152,13 +154,14 @@ def w4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, *, x
                     x_scale.data_ptr() if fp8 else None, qweight.data_ptr(), qweight.stride(0) if n > 1 else words,
                     scales.data_ptr(), scales.stride(0), res.data_ptr(), o_sm)
     lib = _lib.load()
-    need = ctypes.c_size_t(0)
-    st = lib.tv_w4_workspace_size(a, need)
-    if st == 0:
-        if need.value:
+    st = _lib.launch(x.device, lib.tv_w4_linear, a)
+    if st == _lib.TV_ERR_WORKSPACE:      # rows that have to be laid out anew first; nothing was launched
+        need = ctypes.c_size_t(0)
+        st = lib.tv_w4_workspace_size(a, need)
+        if st == 0:
             ws = x.new_empty(need.value, dtype=torch.uint8)
             a.workspace, a.workspace_bytes = ws.data_ptr(), need.value
-        st = _lib.launch(x.device, lib.tv_w4_linear, a)
+            st = _lib.launch(x.device, lib.tv_w4_linear, a)
     if st != 0:
         _lib.check(st, "tv_w4_linear")
     return res
