@@ -1,0 +1,164 @@
+"""The low-bit operators and the residual rule as a program uses them: every
+small row count in every form, calls at once on two streams, graphs replayed
+side by side, batches around each cluster size, and tensors whose element
+offsets pass 32 bits.  Tolerances are those of the operators' own tests."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import test_gpu_residual_accept as ra
+from conftest import cuda_ok
+from test_gpu_w4 import check, problem, to_fp8
+
+pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not cuda_ok(), reason="needs a CUDA device")]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+# one block of 128 k and less, blocks that do not fill a team's warps, ones that do; few and many units;
+# rows that do not fit an SM's shared memory
+@pytest.mark.parametrize("n,k,group", [(16, 32, 32), (17, 128, 64), (100, 480, 32), (2500, 2048, 128),
+                                       (30000, 512, 64), (48, 4224, 128), (33, 14336, 128), (15, 28672, 256)])
+def test_few_rows_in_every_form(n, k, group, dtype):
+    from specverify.runtime import w4_linear
+    for t in range(1, 9):
+        x, q, s = problem(t, n, k, group, dtype, seed=t * n + k)
+        want = w4_linear(x, q, s)
+        check(want, x, q, s)
+        wide = torch.zeros(t, k + 3, dtype=dtype, device="cuda")
+        wide[:, 1:k + 1] = x                     # rows at odd addresses
+        buf = torch.full((2 * t, n + 5), 5.0, dtype=dtype, device="cuda")
+        # both ways of reading x sum in the same order where the same kernel takes them
+        y = w4_linear(wide[:, 1:k + 1], q, s, out=buf[::2, 2:n + 2])
+        check(y, x, q, s)
+        assert bool((buf[1::2] == 5).all()) and bool((buf[:, :2] == 5).all()) and bool((buf[:, n + 2:] == 5).all())
+        x8, xs = to_fp8(x)
+        check(w4_linear(x8, q, s, x_scale=xs), x8, q, s, xs)
+        # a row's result does not hang on the rows beside it
+        if t > 1:
+            assert torch.equal(w4_linear(x[t - 1:], q, s)[0], want[t - 1]) or k > 13000
+
+
+def chain(seed, rows=65):
+    """Residual and norm in 8 bits, the product of it, and the acceptance over its first words."""
+    from specverify.draft import accept_residual
+    from specverify.runtime import add_rms_norm, w4_linear
+    x, q, s = problem(rows, 4096, 2048, 128, torch.bfloat16, seed=seed)
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    r = torch.randn(rows, 2048, device="cuda", generator=g).bfloat16()
+    w = torch.rand(2048, device="cuda", generator=g).bfloat16()
+    draft = torch.randint(0, 4096, (rows,), device="cuda", generator=g)
+    parent = torch.arange(-1, rows - 2, device="cuda") // 2
+    u = torch.rand(rows, device="cuda", generator=g)
+
+    def run():
+        y8, scale, h = add_rms_norm(x, r, w, 1e-5, fp8=True)
+        logits = w4_linear(y8, q, s, x_scale=scale)
+        acc = accept_residual(logits, draft, parent, u)
+        return y8.view(torch.uint8), scale, h, logits, acc.result, acc.next_tokens
+    return run
+
+
+def test_calls_at_once_on_two_streams():
+    runs = [chain(1), chain(2, 9)]
+    want = [[t.clone() for t in run()] for run in runs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(runs[i]())
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
+
+
+def test_graphs_replayed_side_by_side():
+    runs = [chain(3), chain(4)]
+    want = [[t.clone() for t in run()] for run in runs]
+    graphs, outs = [], []
+    for run in runs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(run())
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for out in outs:
+            for t in out:
+                t.zero_()
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for out, w in zip(outs, want):
+            assert all(torch.equal(a, b) for a, b in zip(out, w))
+
+
+@pytest.mark.parametrize("sampled", [False, True])
+# the number of sequences decides how many SMs share one: around every step of that rule
+@pytest.mark.parametrize("b,v", [(1, 40000), (7, 40000), (8, 40000), (15, 33000), (16, 33000), (22, 30000),
+                                 (23, 25000), (34, 18000), (46, 9000), (75, 9000), (160, 5000)])
+def test_batches_around_the_cluster_sizes(b, v, sampled):
+    from specverify.draft import accept_residual
+    logits, draft, parent, u, q = ra.problem(b, 4, v, 2, torch.bfloat16, sampled, seed=b + v)
+    cl, cd, cp, cu, cq = ra.cuda(logits, draft, parent, u, q)
+    ra.check(accept_residual(cl, cd, cp, cu, draft_probs=cq), logits, draft, parent, u, q)
+
+
+def test_drafts_from_the_target_itself():
+    """Draft probabilities that are the target's own, rounded: next to nothing is left of p - q."""
+    from specverify.draft import accept_residual
+    logits, draft, parent, u, _ = ra.problem(6, 5, 3000, 1, torch.float32, True, seed=11)
+    q = torch.softmax(logits, -1)
+    cl, cd, cp, cu, cq = ra.cuda(logits, draft, parent, u, q)
+    acc = accept_residual(cl, cd, cp, cu * 0.999, draft_probs=cq)      # u q < p for all of them: every draft passes
+    assert acc.result[:, 2].tolist() == [5] * 6
+    for dt in (torch.bfloat16, torch.float16):
+        acc = accept_residual(cl, cd, cp, cu, draft_probs=cq.to(dt))
+        assert acc.result[:, 0].tolist() == [0] * 6
+        assert bool((acc.result[:, 3] >= 0).all()) and bool((acc.result[:, 3] < 3000).all())
+
+
+def test_offsets_beyond_32_bits():
+    from specverify.draft import accept_residual
+    from specverify.runtime import add_rms_norm, w4_linear
+    # outputs: 20000 x 128256 elements
+    x, q, s = problem(20000, 128256, 128, 64, torch.bfloat16, seed=1)
+    y = w4_linear(x, q, s)
+    for rows in (slice(0, 40), slice(19960, 20000)):
+        check(y[rows].contiguous(), x[rows], q, s)
+    del y
+    # packed weights: 600000 x 4096 words; rows far apart
+    n, k = 600000, 32768
+    q = torch.randint(-2 ** 31, 2 ** 31, (n, k // 8), dtype=torch.int32, device="cuda")
+    s = torch.full((n, k // 128), 0.004, device="cuda").bfloat16()
+    for t in (2, 20):
+        x = torch.randn(t, k, device="cuda").bfloat16()
+        y = w4_linear(x, q, s)
+        for cols in (slice(0, 200), slice(n - 333, n)):
+            check(y[:, cols].contiguous(), x, q[cols], s[cols])
+    del q, s, y
+    # logits: 70 sequences of 250 rows over 128256 words
+    logits = torch.randn(70, 250, 128256, device="cuda", dtype=torch.bfloat16)
+    draft = torch.randint(0, 128256, (70, 250), device="cuda")
+    parent = (torch.arange(-1, 248, device="cuda") // 3).expand(70, 249).contiguous()
+    u = torch.rand(70, 250, device="cuda")
+    acc = accept_residual(logits, draft, parent, u)
+    for i in (0, 69):
+        one = accept_residual(logits[i].clone(), draft[i], parent[i], u[i])
+        assert torch.equal(acc.result[i], one.result.view(-1))
+    del logits
+    # rows of the norm
+    x = torch.randn(300000, 8192, device="cuda", dtype=torch.bfloat16)
+    r = torch.randn(300000, 8192, device="cuda", dtype=torch.bfloat16)
+    w = torch.rand(8192, device="cuda").bfloat16()
+    y8, scale, h = add_rms_norm(x, r, w, 1e-5, fp8=True)
+    a8, ascale, ah = add_rms_norm(x[-5:].clone(), r[-5:].clone(), w, 1e-5, fp8=True)
+    assert torch.equal(h[-5:], ah) and torch.equal(scale[-5:], ascale)
+    assert torch.equal(y8[-5:].view(torch.uint8), a8.view(torch.uint8))

@@ -98,15 +98,42 @@ def test_w4_linear_checks(lib):
     assert call(x_dtype=3) == -8                                # e4m3 rows need their scales
     assert call(qweight=FAKE + 4) == -3 and call(q_sn=33) == -3 and call(q_sn=28) == -1
     assert call(k=(1 << 20) + 64, q_sn=1 << 20) == -7 and call(n=(1 << 27) + 1) == -7
-    # rows that TMA cannot read are staged: 8 bits, off the 16-byte grid, or overlapping
+    # more than 8 rows that TMA cannot read are staged: 8 bits, off the 16-byte grid, or overlapping
     for kw in (dict(x_dtype=3, x_scale=FAKE), dict(x=FAKE + 2), dict(x_sm=260), dict(x_sm=0)):
+        kw["rows"] = 40
         assert call(**kw) == -5, kw
-        assert call(**kw, workspace=FAKE, workspace_bytes=4 * 256 * 2 - 1) == -5
+        assert call(**kw, workspace=FAKE, workspace_bytes=40 * 256 * 2 - 1) == -5
         assert call(**kw, workspace=FAKE + 8, workspace_bytes=1 << 20) == -3
     assert call(rows=65535 * 128 + 1) == -7
     assert lib.tv_w4_linear(None, None) == -8
     n = ctypes.c_size_t(0)
     assert lib.tv_w4_workspace_size(ctypes.byref(args()), ctypes.byref(n)) == 0 and n.value == 0
-    assert lib.tv_w4_workspace_size(ctypes.byref(args(x_dtype=3)), ctypes.byref(n)) == 0 and n.value == 4 * 256 * 2
+    for rows, need in ((8, 0), (9, 9 * 256 * 2)):
+        assert lib.tv_w4_workspace_size(ctypes.byref(args(x_dtype=3, rows=rows)), ctypes.byref(n)) == 0
+        assert n.value == need
     assert lib.tv_w4_workspace_size(ctypes.byref(args(rows=1, x_sm=0)), ctypes.byref(n)) == 0 and n.value == 0
     assert lib.tv_w4_workspace_size(None, ctypes.byref(n)) == -8
+
+
+def test_structs_match_the_header(tmp_path):
+    """Size and every field's offset of the two argument blocks, as the host C compiler lays them out."""
+    import shutil
+    import subprocess
+    from pathlib import Path
+    if shutil.which("gcc") is None:
+        pytest.skip("no host C compiler")
+    mirrors = {"tv_residual_accept_args": _lib.ResidualAcceptArgs, "tv_w4_args": _lib.W4Args}
+    lines = ["#include <stdio.h>", "#include <stddef.h>", '#include "specverify.h"', "int main(void) {"]
+    want = []
+    for cname, py in mirrors.items():
+        lines.append(f'  printf("%zu\\n", sizeof({cname}));')
+        want.append(ctypes.sizeof(py))
+        for fname, _ in py._fields_:
+            lines.append(f'  printf("%zu\\n", offsetof({cname}, {fname}));')
+            want.append(getattr(py, fname).offset)
+    src, exe = tmp_path / "layout.c", tmp_path / "layout"
+    src.write_text("\n".join(lines + ["  return 0;", "}"]) + "\n")
+    subprocess.run(["gcc", "-I", str(Path(__file__).resolve().parent.parent / "include"), str(src), "-o", str(exe)],
+                   check=True)
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout
+    assert [int(x) for x in out.split()] == want
