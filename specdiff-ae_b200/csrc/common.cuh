@@ -23,6 +23,38 @@ inline int check_launch() {
   return e == cudaSuccess ? TV_OK : record_cuda_error(e);
 }
 
+// ---- kernels that start while the one before them ends ----------------------
+// A kernel launched by launch_early may start once every CTA of its predecessor
+// in the stream has called grid_next or ended; before it touches global memory
+// it calls grid_wait, which returns when the predecessor has completed and its
+// writes are visible.  What comes before that (the launch itself, barriers,
+// tensor memory) is off the critical path.  Every such kernel waits, so
+// completion carries over a chain of them.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// cluster: CTAs along x that form one, 0 or 1 for none.
+template <typename... P>
+int launch_early(void (*kernel)(P...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t st,
+                 const P&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)cluster;
+  at[1].val.clusterDim.y = 1;
+  at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  return e == cudaSuccess ? check_launch() : record_cuda_error(e);
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // ---- element conversions -------------------------------------------------

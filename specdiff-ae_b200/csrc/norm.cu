@@ -181,6 +181,8 @@ __global__ void __launch_bounds__(512) add_rms_norm_kernel(const AddNormArgs a) 
   Chunk<T, VEC> keep[NC];
   Chunk<T, 1> one;
   float ss = 0.f;
+  grid_next();
+  grid_wait();
   // h = T(x + r), stored and squared
   auto join = [&](auto& u, const auto& v, int c) {
     constexpr int N = sizeof(u) / sizeof(T);
@@ -321,8 +323,7 @@ __global__ void __launch_bounds__(512) add_rms_norm_kernel(const AddNormArgs a) 
 
 template <typename T, bool FP8, int VEC, int NC, bool WIDE, bool SHIFT>
 int launch_add_norm(const AddNormArgs& a, int rows, int threads, cudaStream_t st) {
-  add_rms_norm_kernel<T, FP8, VEC, NC, WIDE, SHIFT><<<rows, threads, 0, st>>>(a);
-  return check_launch();
+  return launch_early(add_rms_norm_kernel<T, FP8, VEC, NC, WIDE, SHIFT>, dim3((unsigned)rows), threads, 0, 0, st, a);
 }
 
 enum AddNormLayout { kRowsAligned, kRowsShifted, kRowsAny };

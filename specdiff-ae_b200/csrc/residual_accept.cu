@@ -159,7 +159,8 @@ template <typename E>
 __global__ void __launch_bounds__(kStatThreads) row_stats_kernel(const Args a) {
   constexpr int VEC = 16 / sizeof(E);
   constexpr int U = kChunkBytes / (16 * kStatThreads);
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  grid_wait();
+  grid_next();        // not before: stage 2 reads the tree without a wait of its own
   const int row = blockIdx.y, b = blockIdx.z;
   if (a.counts && row >= a.counts[b]) return;
   const int lo = blockIdx.x * a.chunk;
@@ -300,7 +301,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) walk_kernel(const Args a) {
   // 2. each node's maximum and normaliser from its chunks' pairs, five nodes'
   // loads at a time (a tree of 64 and its root in one turn)
   constexpr int kNodes = 5;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  grid_wait();
   for (int i0 = warp; i0 < n; i0 += kNodes * kWalkWarps) {
     float m[kNodes], pm[kNodes];
     double ps[kNodes], s[kNodes];
@@ -687,29 +688,14 @@ int launch_walk(const Args& a, int batch, size_t smem, cudaStream_t st) {
     const int rc = ensure_wide_cluster<E, Q, SAMPLED>();
     if (rc != TV_OK) return rc;
   }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(size, batch);
-  cfg.blockDim = dim3(kWalkThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = size;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
   // stage 2 starts while stage 1 ends and waits for its results on the device
-  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, walk_kernel<E, Q, SAMPLED>, a);
-  return e == cudaSuccess ? check_launch() : record_cuda_error(e);
+  return launch_early(walk_kernel<E, Q, SAMPLED>, dim3((unsigned)size, (unsigned)batch), kWalkThreads, smem, size, st, a);
 }
 
 template <typename E>
 int launch(const Args& a, int probs_dtype, int batch, size_t smem, cudaStream_t st) {
-  row_stats_kernel<E><<<dim3(a.chunks, a.rows, batch), kStatThreads, 0, st>>>(a);
-  const int rc = check_launch();
+  const int rc = launch_early(row_stats_kernel<E>, dim3((unsigned)a.chunks, (unsigned)a.rows, (unsigned)batch),
+                              kStatThreads, 0, 0, st, a);
   if (rc != TV_OK) return rc;
   if (!a.probs) return launch_walk<E, float, false>(a, batch, smem, st);
   if (probs_dtype == TV_F32) return launch_walk<E, float, true>(a, batch, smem, st);

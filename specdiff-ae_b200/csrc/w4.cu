@@ -131,6 +131,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   Bars* bars = reinterpret_cast<Bars*>(smem + kRing);
   volatile int* abort = &bars->abort;
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  grid_next();
   const int rank = blockIdx.x % p.split;
   const int n0 = blockIdx.x / p.split * kRows;
   const int t0 = blockIdx.y * p.tokens;
@@ -177,6 +178,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       mbar_fence_init();
     }
     __syncwarp();
+    grid_wait();
     while (pi < count && pi < ring) issue();
   } else if (warp == 1) {
     if (lane == 0) {
@@ -196,6 +198,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars->tmem;
+  grid_wait();
 
   if (wt || warp == 2) {
     while (pi < count) {
@@ -439,6 +442,8 @@ __host__ __device__ constexpr int padded_k(int k) { return (k + 63) / 64 * 64; }
 
 template <typename X, typename T>
 __global__ void __launch_bounds__(256) w4_stage_kernel(const X* x, int64_t x_sm, T* y, int rows, int k) {
+  grid_next();
+  grid_wait();
   const int chunks = padded_k(k) / 8;
   const int64_t total = (int64_t)rows * chunks;
   for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
@@ -498,20 +503,8 @@ int launch_kernel(const CUtensorMap& mw, const CUtensorMap& mx, const W4Params& 
                   cudaStream_t st) {
   const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(w4_kernel<T, SCALES>), kSmem);
   if (rc != TV_OK) return rc;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(blocks_n * p.split), (unsigned)blocks_t);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kSmem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = p.split;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = p.split > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, w4_kernel<T, SCALES>, mw, mx, p);
-  return e == cudaSuccess ? check_launch() : record_cuda_error(e);
+  return launch_early(w4_kernel<T, SCALES>, dim3((unsigned)(blocks_n * p.split), (unsigned)blocks_t), kThreads, kSmem,
+                      p.split, st, mw, mx, p);
 }
 
 template <typename T>
@@ -522,12 +515,12 @@ int launch_w4(const tv_w4_args* a, cudaStream_t st) {
     T* y = static_cast<T*>(a->workspace);
     const int64_t chunks = (int64_t)a->rows * (padded_k(a->k) / 8);
     const int blocks = (int)(chunks / 256 + 1 < 4 * kNumSMs ? chunks / 256 + 1 : 4 * kNumSMs);
-    if (a->x_dtype == TV_E4M3)
-      w4_stage_kernel<__nv_fp8_e4m3, T><<<blocks, 256, 0, st>>>(static_cast<const __nv_fp8_e4m3*>(a->x), a->x_sm, y,
-                                                                a->rows, a->k);
-    else
-      w4_stage_kernel<T, T><<<blocks, 256, 0, st>>>(static_cast<const T*>(a->x), a->x_sm, y, a->rows, a->k);
-    const int rc = check_launch();
+    const int rc =
+        a->x_dtype == TV_E4M3
+            ? launch_early(w4_stage_kernel<__nv_fp8_e4m3, T>, dim3((unsigned)blocks), 256, 0, 0, st,
+                           static_cast<const __nv_fp8_e4m3*>(a->x), a->x_sm, y, a->rows, a->k)
+            : launch_early(w4_stage_kernel<T, T>, dim3((unsigned)blocks), 256, 0, 0, st, static_cast<const T*>(a->x),
+                           a->x_sm, y, a->rows, a->k);
     if (rc != TV_OK) return rc;
     x = y;
     x_sm = padded_k(a->k);

@@ -149,6 +149,8 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const Params p) {
       at_unit();
     }
   };
+  grid_next();
+  grid_wait();
   Batch ping{}, pong{};
   int unit = ahead.unit, b = lo;
   at_unit();
@@ -255,8 +257,7 @@ template <typename T, typename X, bool FOUR>
 int start(const Params& p, int grid, size_t smem, cudaStream_t st) {
   const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(w4_rows_kernel<T, X, FOUR>), (int)smem);
   if (rc != TV_OK) return rc;
-  w4_rows_kernel<T, X, FOUR><<<grid, kThreads, smem, st>>>(p);
-  return check_launch();
+  return launch_early(w4_rows_kernel<T, X, FOUR>, dim3((unsigned)grid), kThreads, smem, 0, st, p);
 }
 
 template <typename T, typename X>

@@ -160,5 +160,12 @@ def test_offsets_beyond_32_bits():
     w = torch.rand(8192, device="cuda").bfloat16()
     y8, scale, h = add_rms_norm(x, r, w, 1e-5, fp8=True)
     a8, ascale, ah = add_rms_norm(x[-5:].clone(), r[-5:].clone(), w, 1e-5, fp8=True)
-    assert torch.equal(h[-5:], ah) and torch.equal(scale[-5:], ascale)
-    assert torch.equal(y8[-5:].view(torch.uint8), a8.view(torch.uint8))
+    # h is the same element by element.  The sum of 8192 squares runs over 128 or 512 threads, as the number of rows
+    # decides: in any order it is off by less than 8192 * 2^-24 of itself, so the two inverse roots, and with them
+    # the scales, differ by less than 2^-11 and a few roundings (2^-20).  8-bit values are off by half a step each:
+    # 2^-4 of the value, or 2^-10 of the scale below the normal range.
+    assert torch.equal(h[-5:], ah)
+    assert bool(((scale[-5:] - ascale).abs() <= (2.0 ** -11 + 2.0 ** -20) * ascale).all())
+    a, b = y8[-5:].double() * scale[-5:, None].double(), a8.double() * ascale[:, None].double()
+    assert bool(((a - b).abs() <= (2 * 2.0 ** -4 + 2.0 ** -10) * torch.maximum(a.abs(), b.abs())
+                 + 2.0 ** -9 * ascale[:, None]).all())
