@@ -544,10 +544,12 @@ int launch_w4(const tv_w4_args* a, cudaStream_t st) {
   const int blocks_t = (a->rows + p.tokens - 1) / p.tokens;
   const int64_t tiles = (int64_t)((a->n + kRows - 1) / kRows) * blocks_t;
   const int stages = (a->k + kStageK - 1) / kStageK;
-  // the largest cluster of which that many run at once, two CTAs per SM (half
-  // of these pairs as the occupancy query reports them: clusters do not span
-  // processor groups)
-  constexpr int fit[kMaxCluster + 1] = {0, 296, 148, 90, 66, 52, 44, 30, 30};
+  // the largest cluster of which that many run at once, two CTAs per SM: by the
+  // time over the number of tiles (8192 k, 33 rows), which steps from 11.4 to 17.1
+  // us behind 33 clusters of 8, 12.3 to 18.7 behind 37 of 7, and so on behind 45
+  // of 6, 56 of 5, 70 of 4 and 92 of 3 (clusters do not span processor groups).
+  // A little less here, as the groups' sizes differ from one GPU to the next.
+  constexpr int fit[kMaxCluster + 1] = {0, 296, 148, 90, 68, 54, 44, 36, 32};
   p.split = 1;
   for (int c = 2; c <= kMaxCluster; ++c)
     if (tiles <= fit[c] && stages >= c) p.split = c;
