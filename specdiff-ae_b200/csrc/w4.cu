@@ -178,6 +178,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       mbar_fence_init();
     }
     __syncwarp();
+    // the first weights may come to L2 before the predecessor's end: what it
+    // still writes is seen there all the same
+    if (wt && lane < min(count, ring)) tma_prefetch_2d(&tmw, (kb0 + lane) * (kStageK / 2), n0);
     grid_wait();
     while (pi < count && pi < ring) issue();
   } else if (warp == 1) {

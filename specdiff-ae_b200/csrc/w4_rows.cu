@@ -150,6 +150,13 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const Params p) {
     }
   };
   grid_next();
+  // the first weights may come to L2 before the predecessor's end: what it
+  // still writes is seen there all the same
+  if (ahead.unit < p.units && lane < kM && lo < hi) {
+    const int bytes = min(min(lo + 2 * kBatch, hi) * kBlockK, p.k) / 2 - lo * (kBlockK / 2);
+    const uint32_t* at = p.q + (int64_t)min(ahead.unit * kM + lane, p.n - 1) * p.q_sn + lo * (kBlockK / 8);
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(at), "r"(bytes) : "memory");
+  }
   grid_wait();
   Batch ping{}, pong{};
   int unit = ahead.unit, b = lo;
