@@ -28,9 +28,17 @@
 // draws in ten thousand.  Stage 2 therefore carries weights and sums as
 // unevaluated pairs of floats (about 2^-36 a weight, one draw in a million);
 // FP64 instructions would do too, but run at 1/24 of the fp32 rate here (49 us
-// for one row of 128256 words on eight SMs, against 4).  Stage 1's normaliser
-// (fp32 exponentials, summed in 64 bits) enters only the few comparisons of a
-// child's probability.
+// for one row of 128256 words on eight SMs; the pairs take 4 on sixteen).
+// Stage 1's normaliser (fp32 exponentials, summed in 64 bits) enters only the
+// few comparisons of a child's probability.
+//
+// A tree of 65 over 128256 words takes 18.0 us: about 6 for stage 1 (2.5 at the
+// measured HBM rate), then 2 to join the pairs, 2 for the walk, 4 for the pass
+// over the ending row, 2 for the draw, each a few dependent round trips.  32
+// sampled trees of 9 take 62 us, stage 1 19 of them (11.3 at the HBM rate): a pass
+// over 32064 words an SM is 9 us of issue (some 65 instructions a word), and the
+// sequence with the most rejections makes three or four.  Folding the first two
+// passes into one by correcting stage 1's normaliser afterwards took 60.4.
 #include <cooperative_groups.h>
 
 #include <atomic>

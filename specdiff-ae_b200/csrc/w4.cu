@@ -26,12 +26,14 @@
 // What bounds it: an MMA of 128 rows x 16 k takes about 37 cycles however few
 // the tokens (its A operand's way out of tensor memory), so a stage is 0.32 us of
 // an SM's tensor pipe, and two CTAs there were seen to take 0.37 a stage: 65
-// rows x 28672 x 4096 spend 12 of 23.5 us in that (16 stages, two CTAs on half of
-// the SMs, one on the others), 3.3 until the first weights are there and 4 from
-// the last MMA to the end.  128 rows x 128256 x 4096: 119 us, 1.13 PFLOP/s.
+// rows x 28672 x 4096 (21.7 us) spend 12 us in that (16 stages, two CTAs on half
+// of the SMs, one on the others), the rest on the way to the first weights (2-3)
+// and from the last MMA to the stored rows (2).  128 rows x 128256 x 4096: 119 us,
+// 1.13 PFLOP/s.  Where k is split, 65 rows x 4096 x 14336 take 15.5 us, 4 of them
+// behind the last MMA: two cluster barriers and the sums' way between SMs.
 // Tiles of 256 weight rows with k cut evenly over the SMs balance better and were
-// slower, as were pairs of CTAs splitting k (37 us): partial sums cost more
-// than idle SMs.  Weights as the B operand would pad the tokens to 128.
+// slower, as were pairs of CTAs splitting k (37 us at 28672 x 4096): partial sums
+// cost more than idle SMs.  Weights as the B operand would pad the tokens to 128.
 #include <cooperative_groups.h>
 #include <cuda.h>
 #include <cuda_fp8.h>

@@ -14,15 +14,19 @@
 // per warp: each block's registers are loaded anew, eight blocks ahead, as soon
 // as it is used.  A team's sums meet in shared memory and are added in order.
 //
-// One row x 28672 x 4096 takes 17.2 us, 8 rows 18.6 (9.0 at the measured HBM
-// rate; the loads alone 13.0): issue comes next to HBM, about 140 instructions
-// a warp for 2048 weights, 72 of them the unpacking.  Two CTAs of eight warps
-// an SM, up to 16 units on one SM and 8 on another, took 18.8 and 21.9; one
-// batch of four blocks in flight instead of two 18.5 and 20.3 at teams of four.
-// Whole units a warp (no split of k) run 18.9 at 8 x 28672 x 4096, but 10.4 for
-// 7.7 at 8 x 6144 x 4096; teams of eight 19.5 and 8.1.  The tcgen05 kernel has a
-// pipeline of five roles to start and drain: 21.4 at one row x 28672 x 4096, 9.2
-// against 4.8 at 4096 x 4096.
+// The first eight blocks come to L2 by one bulk request a row while the kernel
+// before this one ends (16.3 -> 15.1 us at one row x 28672 x 4096, 18.0 -> 16.6 at
+// 8); requests further ahead, all along the way, were slower (18.2 and 19.7).
+//
+// One row x 28672 x 4096 takes 15.1 us, 8 rows 16.6 (9.0 at the measured HBM
+// rate): issue comes next to HBM, about 140 instructions a warp for 2048 weights,
+// 72 of them the unpacking, 5.7 us of every scheduler.  Before the bulk requests:
+// two CTAs of eight warps an SM, up to 16 units on one SM and 8 on another, took
+// 18.8 and 21.7 where this form took 17.2 and 18.4; one batch of four blocks in
+// flight instead of two 19.2 and 20.3.  Whole units a warp (no split of k) took 18.9
+// at 8 x 28672 x 4096, but 10.4 for 7.7 at 8 x 6144 x 4096; teams of eight 19.5 and
+// 8.1.  16 rows (two tiles of N) took 10.2 for the tcgen05 kernel's 10.5 at 6144 x
+// 4096 and 26.1 for 22.4 at 28672 x 4096, so that takes over at 9.
 #include <cuda_fp8.h>
 
 #include <type_traits>
@@ -40,8 +44,8 @@ constexpr int kTeam = 4;                // warps that share 16 weight rows
 constexpr int kTeams = kWarps / kTeam;
 constexpr int kM = 16;                  // weight rows per unit
 constexpr int kBlockK = 128;
-constexpr int kBatch = 4;               // blocks in flight
-constexpr int kMaxRows = 8;             // N of m16n8k16; with two of them the tcgen05 kernel is the faster
+constexpr int kBatch = 4;               // blocks of a batch; two batches are in flight
+constexpr int kMaxRows = 8;             // N of m16n8k16
 constexpr int kMaxSmem = 220 * 1024;
 
 struct Params {
