@@ -196,6 +196,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       mbar_fence_init();
     }
     __syncwarp();
+    // not before: a predecessor may still want tensor memory itself, and would
+    // wait for what this CTA held while it waits for the predecessor
+    grid_wait();
     tmem_alloc(&bars->tmem, kTmemCols);
     tmem_relinquish();
   }
