@@ -449,7 +449,7 @@ class SpecDecodeModel:
             hidden, feats = self.verify(ids, pos, tree["mask_bits"], start)
         ev[2].record()
         if acceptance == "residual":
-            gen = torch.Generator(device=self.device).manual_seed((seed << 20) + offset)
+            gen = torch.Generator(device=self.device).manual_seed(((seed << 20) + offset) & (2 ** 63 - 1))
             uniform = torch.rand(ids.numel(), device=self.device, generator=gen)
             acc = accept_residual(hidden @ self.lm_head.t(), ids, parent, uniform, temperature=temperature)
         else:

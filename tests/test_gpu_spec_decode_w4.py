@@ -138,3 +138,11 @@ def test_arguments():
     with pytest.raises(ValueError):
         m.diffspec_generate(PROMPT, 4, 8, 4, acceptance="other")
     assert isinstance(m, SpecDecodeModel)
+
+
+@pytest.mark.parametrize("seed", [0, 2 ** 45 + 3, 2 ** 62])
+def test_residual_rule_takes_large_seeds(seed):
+    m = _model()
+    a = m.diffspec_generate(PROMPT, 4, 8, 4, temperature=1.0, seed=seed, max_steps=2, acceptance="residual")
+    b = m.diffspec_generate(PROMPT, 4, 8, 4, temperature=1.0, seed=seed, max_steps=2, acceptance="residual")
+    assert a["steps"] >= 1 and a["tokens"] == b["tokens"]
