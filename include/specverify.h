@@ -354,7 +354,7 @@ typedef struct tv_residual_accept_args {
   int32_t probs_dtype;
   const void* probs;             /* optional [batch][rows][vocab]           */
   int64_t probs_sb, probs_sm;
-  float temperature;
+  double temperature;            /* 64 bits: a float's 2^-24 would move every weight of a row the same way */
   int64_t* next_tokens;
   int64_t* result;
   void* workspace;

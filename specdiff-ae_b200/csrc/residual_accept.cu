@@ -732,7 +732,7 @@ int tv_residual_accept(const tv_residual_accept_args* a, void* stream) {
   if (a->rows > 1024 || a->batch > 65535 || a->vocab > (1 << 30)) return TV_ERR_UNSUPPORTED;
   if (a->logits_dtype < TV_BF16 || a->logits_dtype > TV_F32) return TV_ERR_DTYPE;
   if (a->probs && (a->probs_dtype < TV_BF16 || a->probs_dtype > TV_F32)) return TV_ERR_DTYPE;
-  if (!(a->temperature >= 1e-20f) || !(a->temperature <= 1e20f)) return TV_ERR_INPUT;   // log2(e) / T as a float
+  if (!(a->temperature >= 1e-20) || !(a->temperature <= 1e20)) return TV_ERR_INPUT;   // log2(e) / T as a float
   if (a->batch == 0) return TV_OK;
   if (!a->logits || !a->draft || !a->uniform || !a->next_tokens || !a->result) return TV_ERR_NULL;
   if (a->rows > 1 && !a->parent) return TV_ERR_NULL;
@@ -758,7 +758,7 @@ int tv_residual_accept(const tv_residual_accept_args* a, void* stream) {
   k.probs = a->probs;
   k.q_sb = a->probs_sb;
   k.q_sm = a->probs_sm;
-  const double c = 1.4426950408889634074 / (double)a->temperature;
+  const double c = 1.4426950408889634074 / a->temperature;
   k.c_hi = (float)c;
   while ((double)k.c_hi >= c) k.c_hi = nextafterf(k.c_hi, 0.f);
   k.c_lo = (float)(c - (double)k.c_hi);

@@ -31,8 +31,8 @@ class SpecVerifyError(RuntimeError):
                          + (f" [{last_cuda_error()}]" if status == -4 else ""))
 
 
-c_i32, c_i64, c_f32, c_u64, c_size, c_vp = (ctypes.c_int32, ctypes.c_int64, ctypes.c_float,
-                                            ctypes.c_uint64, ctypes.c_size_t, ctypes.c_void_p)
+c_i32, c_i64, c_f32, c_f64, c_u64, c_size, c_vp = (ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_double,
+                                                   ctypes.c_uint64, ctypes.c_size_t, ctypes.c_void_p)
 
 
 class AttnArgs(ctypes.Structure):
@@ -107,7 +107,7 @@ class ResidualAcceptArgs(ctypes.Structure):
         ("draft", c_vp), ("draft_sb", c_i64), ("parent", c_vp), ("parent_sb", c_i64),
         ("counts", c_vp), ("uniform", c_vp), ("uniform_sb", c_i64),
         ("probs_dtype", c_i32), ("probs", c_vp), ("probs_sb", c_i64), ("probs_sm", c_i64),
-        ("temperature", c_f32), ("next_tokens", c_vp), ("result", c_vp),
+        ("temperature", c_f64), ("next_tokens", c_vp), ("result", c_vp),
         ("workspace", c_vp), ("workspace_bytes", c_size),
     ]
 

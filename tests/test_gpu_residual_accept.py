@@ -362,3 +362,33 @@ def test_refusals():
     for args, kw in bad:
         with pytest.raises(SpecVerifyError):
             accept_residual(*args, **{**ok, **kw})
+
+
+@pytest.mark.parametrize("t", [0.7, 0.9, 1.3])
+def test_draws_next_to_borders_at_temperatures_that_no_float_holds(t):
+    """Draws beside the borders of softmax(logits / t) with t in 64 bits.  A temperature rounded to 32 bits is off by
+    2^-26 to 2^-24 of itself and moves the borders by some 2^-29 of the sum, all of a row the same way.  The uniform
+    numbers here lie between 2^-32 and 2^-29 of the sum from a border; the kernel's own error is that of its weights
+    (2^-36 each) and of their sum (the pairs' l parts, below 2^-40), the 80-bit CDF's is below 2^-46."""
+    from specverify.draft import accept_residual
+    v = 128256
+    g = torch.Generator().manual_seed(int(100 * t))
+    logits = (3.0 * torch.randn(1, 1, v, generator=g)).to(torch.float16)
+    x = logits[0, 0].double().numpy().astype(np.longdouble)
+    cdf = np.cumsum(np.exp((x - x.max()) / np.longdouble(t)))
+    cdf /= cdf[-1]
+    u = cdf[:-1].astype(np.float32)
+    far = np.abs(u.astype(np.longdouble) - cdf[:-1])
+    u = u[(far > 2.0 ** -32) & (far < 2.0 ** -29) & (u < 1)]
+    assert len(u) > 2000
+    # numbers near 0 are finer than the borders' errors: only the nearest border decides how far one is
+    want = np.searchsorted(cdf, u.astype(np.longdouble), side="right")
+    near = np.minimum(np.abs(cdf[np.minimum(want, v - 1)] - u), np.abs(u - cdf[np.maximum(want - 1, 0)]))
+    u, want = u[near > 2.0 ** -32], want[near > 2.0 ** -32]
+    b = len(u)
+    acc = accept_residual(logits.cuda().expand(b, 1, v), torch.zeros(b, 1, dtype=torch.int64, device="cuda"),
+                          torch.zeros(b, 0, dtype=torch.int64, device="cuda"), torch.from_numpy(u)[:, None].cuda(),
+                          temperature=t)
+    assert (acc.result[:, 0] == 0).all()
+    wrong = int((acc.result[:, 3].cpu().numpy() != want).sum())
+    assert wrong == 0, (wrong, b)
