@@ -449,8 +449,7 @@ class SpecDecodeModel:
             hidden, feats = self.verify(ids, pos, tree["mask_bits"], start)
         ev[2].record()
         if acceptance == "residual":
-            gen = torch.Generator(device=self.device).manual_seed(((seed << 20) + offset) & (2 ** 63 - 1))
-            uniform = torch.rand(ids.numel(), device=self.device, generator=gen)
+            uniform = self._uniform(ids.numel(), seed, offset)
             acc = accept_residual(hidden @ self.lm_head.t(), ids, parent, uniform, temperature=temperature)
         else:
             acc = accept_from_hidden(hidden, self.lm_head, ids, parent, pos,
@@ -459,6 +458,14 @@ class SpecDecodeModel:
         self._compact(start, acc, ids.numel())
         ev[3].record()
         return acc, feats, ev
+
+    def _uniform(self, n: int, seed: int, offset: int) -> torch.Tensor:
+        """Step ``offset``'s uniform numbers: Philox keyed by all 64 bits of
+        ``seed``, counted on from ``offset`` (a step of n <= 1024 numbers takes 4
+        of a thread's counter, so 256 keep the steps apart)."""
+        gen = torch.Generator(device=self.device).manual_seed(int(seed) & (2 ** 64 - 1))
+        gen.set_offset((int(offset) << 8) & (2 ** 63 - 1))
+        return torch.rand(n, device=self.device, generator=gen)
 
     def _draft_graphed(self, root, root_feat, start: int, width: int, depth: int):
         """draft_tree replayed from a CUDA graph captured on first use (static

@@ -146,3 +146,28 @@ def test_residual_rule_takes_large_seeds(seed):
     a = m.diffspec_generate(PROMPT, 4, 8, 4, temperature=1.0, seed=seed, max_steps=2, acceptance="residual")
     b = m.diffspec_generate(PROMPT, 4, 8, 4, temperature=1.0, seed=seed, max_steps=2, acceptance="residual")
     assert a["steps"] >= 1 and a["tokens"] == b["tokens"]
+
+
+def test_residual_rule_draws_other_numbers_for_every_seed_and_step(monkeypatch):
+    """Seeds that agree in their low 43 bits, and a step number that runs past 20 bits: no number is shared (nine of
+    24 bits each: by chance two sets have one in common once in 2^17), and the same seed and step repeat theirs."""
+    from specverify.draft import spec_decode
+    m = _model()
+    root = m.fill_context(PROMPT, seed=5)
+    feat = torch.zeros(1, 3 * 512, device="cuda", dtype=m.dtype)
+    seen = []
+    rule = spec_decode.accept_residual
+
+    def record(logits, draft, parent, uniform, **kw):
+        seen.append(uniform.tolist())
+        return rule(logits, draft, parent, uniform, **kw)
+
+    monkeypatch.setattr(spec_decode, "accept_residual", record)
+    runs = [(0, 0), (3, 0), (2 ** 45 + 3, 0), (2 ** 62, 0), (2 ** 63 + 3, 0), (-1, 0), (1, 0), (0, 1), (0, 2 ** 20),
+            (0, 2 ** 32), (2 ** 43, 0)]
+    for seed, offset in runs + runs[:1]:
+        m.step(torch.tensor([root], device="cuda"), feat, PROMPT, 2, 4, 1.0, seed, offset, acceptance="residual")
+    assert seen[-1] == seen[0] and len(seen[0]) == 9
+    for i in range(len(runs)):
+        for j in range(i):
+            assert not set(seen[i]) & set(seen[j]), (runs[i], runs[j])
