@@ -609,7 +609,9 @@ int tv_add_rms_norm(const void* x, int64_t x_row_stride, const void* residual, i
  * workspace: tv_w4_workspace_size bytes, 16-byte aligned; 0 bytes unless x has to
  * be laid out anew first (more rows than 8, or than fit shared memory, in e4m3,
  * off the 16-byte grid or with k no multiple of 64).  Without one such a call
- * returns TV_ERR_WORKSPACE before any launch. */
+ * returns TV_ERR_WORKSPACE before any launch.
+ * Waits on the device are bounded (2^32 SM clocks, about 2 s).  One that runs out
+ * leaves NaN in its tile of out and a positive code in *status (if given). */
 typedef struct tv_w4_args {
   int32_t x_dtype, out_dtype;
   int32_t rows, n, k, group;
@@ -624,6 +626,7 @@ typedef struct tv_w4_args {
   int64_t o_sm;
   void* workspace;
   size_t workspace_bytes;
+  int32_t* status;               /* optional device word, zeroed by the caller */
 } tv_w4_args;
 
 int tv_w4_workspace_size(const tv_w4_args* args, size_t* bytes);

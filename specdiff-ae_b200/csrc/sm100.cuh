@@ -101,6 +101,13 @@ __device__ __forceinline__ bool mbar_wait_suspend(uint64_t* bar, uint32_t parity
   }
 }
 
+// After a wait that ran out: the CTA's other waits end early, and the caller's
+// status word, if there is one, keeps the first code.
+__device__ __forceinline__ void give_up(volatile int* abort, int* status, int code) {
+  *abort = 1;
+  if (status) atomicCAS(status, 0, code);
+}
+
 // One lane of a converged warp.  Unlike a test of the lane index this leaves
 // the control flow around it uniform, so the operands of tcgen05.mma, which
 // the hardware takes from uniform registers, need no per-use transfer.

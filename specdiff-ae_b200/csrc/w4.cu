@@ -86,6 +86,7 @@ struct W4Params {
   int tokens;                  // N of the MMA: tokens per CTA, a multiple of 16
   int w_stages, x_stages, x_bytes;
   int split;                   // CTAs of a cluster
+  int* status;                 // optional
   uint32_t zero;               // 0, unknown to the compiler
   uint32_t group_magic;        // k / group = (k / 32) * magic >> 32; 0: group 32
 };
@@ -97,6 +98,11 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* v) {
         "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
       : "r"(taddr));
 }
+
+// What ran out, in *status: a producer's wait for a free stage, the MMA
+// issuer's for its operands, the unpacking's for weights or a free buffer, the
+// epilogue's for the accumulator.
+enum { kGaveUpLoads = 1, kGaveUpMma, kGaveUpUnpack, kGaveUpSums };
 
 // The address of a shared-memory word in another CTA of the cluster, and a load
 // from there; 0 where `in` is false.
@@ -211,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (wt || warp == 2) {
     while (pi < count) {
       if (!__all_sync(0xffffffffu, mbar_wait_suspend(&empty[ps], pph, abort))) {
-        bars->abort = 1;
+        give_up(abort, p.status, kGaveUpLoads);
         break;
       }
       issue();
@@ -249,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         xph ^= 1;
       }
     }
-    if (!ok) bars->abort = 1;
+    if (!ok) give_up(abort, p.status, kGaveUpMma);
     else if (elected) tc_commit(&bars->done);
   } else if (warp >= kDequantWarp) {
     const int g = (warp - kDequantWarp) >> 2;
@@ -365,10 +371,10 @@ __global__ void __launch_bounds__(kThreads, 2)
         ph ^= 1;
       }
     }
-    if (!ok) bars->abort = 1;
+    if (!ok) give_up(abort, p.status, kGaveUpUnpack);
     // ---- epilogue
     ok = __all_sync(0xffffffffu, mbar_wait_suspend(&bars->done, 0, abort)) && ok;
-    if (!ok) bars->abort = 1;
+    if (!ok) give_up(abort, p.status, kGaveUpSums);
     tc_fence_after();
     T* out = static_cast<T*>(p.out);
     float* part = reinterpret_cast<float*>(smem);        // [token][weight row], once both rings are drained
@@ -403,6 +409,10 @@ __global__ void __launch_bounds__(kThreads, 2)
   __syncwarp();
   if (p.split > 1) {
     cg::cluster_group cluster = cg::this_cluster();
+    // a CTA that gave up leaves NaNs, written once its last loads have landed
+    if (__syncthreads_or(*abort))
+      for (int e = threadIdx.x; e < p.tokens * kRows; e += kThreads)
+        reinterpret_cast<float*>(smem)[e] = __int_as_float(0x7fc00000);
     cluster.sync();
     if (warp >= kDequantWarp) {
       const int tid = threadIdx.x - kDequantWarp * 32;
@@ -412,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int k = 0; k < kMaxCluster; ++k) part[k] = map_rank(smem_u32(smem) + r * 4, min(k, p.split - 1));
       // this CTA's tokens, one of every p.split; three at a time, all of their
-      // parts on their way together.  A CTA that gave up left NaNs.
+      // parts on their way together
       const int step = p.split * 2;
 #pragma unroll 1
       for (int j0 = rank + p.split * (tid / kRows); j0 < p.tokens; j0 += 3 * step) {
@@ -549,6 +559,7 @@ int launch_w4(const tv_w4_args* a, cudaStream_t st) {
   p.x_stages = p.tokens <= 16 ? 6 : p.tokens <= 48 ? 4 : p.tokens <= 80 ? 3 : 2;
   p.w_stages = (kRing - p.x_stages * p.x_bytes) / kWStage;
   p.group_magic = group_magic(a->group);
+  p.status = a->status;
   const int blocks_t = (a->rows + p.tokens - 1) / p.tokens;
   const int64_t tiles = (int64_t)((a->n + kRows - 1) / kRows) * blocks_t;
   const int stages = (a->k + kStageK - 1) / kStageK;

@@ -118,7 +118,7 @@ class W4Args(ctypes.Structure):
         ("x_dtype", c_i32), ("out_dtype", c_i32), ("rows", c_i32), ("n", c_i32), ("k", c_i32), ("group", c_i32),
         ("x", c_vp), ("x_sm", c_i64), ("x_scale", c_vp), ("qweight", c_vp), ("q_sn", c_i64),
         ("scales", c_vp), ("s_sn", c_i64), ("out", c_vp), ("o_sm", c_i64),
-        ("workspace", c_vp), ("workspace_bytes", c_size),
+        ("workspace", c_vp), ("workspace_bytes", c_size), ("status", c_vp),
     ]
 
 

@@ -161,6 +161,7 @@ class SpecDecodeModel:
             raise ValueError("act_fp8 needs weight_bits=4")
         s = self.shape = shape
         self.weight_bits, self.act_fp8 = weight_bits, act_fp8
+        self.status = torch.zeros(1, dtype=torch.int32, device=device)      # of the 4-bit products
         self.device, self.dtype, self.page = device, dtype, page_size
         d = s.head_dim
 
@@ -268,17 +269,20 @@ class SpecDecodeModel:
             out = add_rms_norm(a, x, w, s.rms_eps, fp8=self.act_fp8, residual_out=x)
             return (out[0], out[1]) if self.act_fp8 else (out[0], None)
 
+        def product(a, w, **kw):
+            return w4_linear(a, *w, status=self.status, **kw)
+
         if li < 0:
             torch.index_select(self.embed, 0, vs["ids"], out=x)
             L = self.layers[0]
-            w4_linear(rms_norm(x, L.ln1, s.rms_eps), *L.wqkv, out=vs["qkv"])
+            product(rms_norm(x, L.ln1, s.rms_eps), L.wqkv, out=vs["qkv"])
             return
         L = self.layers[li]
-        y, scale = add_norm(w4_linear(vs["o"].view(x.shape[0], -1), *L.wo), L.ln2)
-        down = w4_linear(silu_mul(w4_linear(y, *L.wgu, x_scale=scale), s.ffn), *L.wdown)
+        y, scale = add_norm(product(vs["o"].view(x.shape[0], -1), L.wo), L.ln2)
+        down = product(silu_mul(product(y, L.wgu, x_scale=scale), s.ffn), L.wdown)
         if li + 1 < s.layers:
             y, scale = add_norm(down, self.layers[li + 1].ln1)
-            w4_linear(y, *self.layers[li + 1].wqkv, x_scale=scale, out=vs["qkv"])
+            product(y, self.layers[li + 1].wqkv, x_scale=scale, out=vs["qkv"])
         else:
             vs["hidden"].copy_(add_rms_norm(down, x, self.norm, s.rms_eps, residual_out=x)[0])
         if li in s.feature_layers:
@@ -531,6 +535,7 @@ class SpecDecodeModel:
         phases = {"draft_ms": 0.0, "verify_ms": 0.0, "accept_compact_ms": 0.0}
         accepted = []
         steps = 0
+        self.status.zero_()
         torch.cuda.synchronize()
         t0 = time.perf_counter()
         evs = []
@@ -554,6 +559,9 @@ class SpecDecodeModel:
             out[-1] = int(nxt.item())
         torch.cuda.synchronize()
         wall = time.perf_counter() - t0
+        code = int(self.status.item())
+        if code != 0:
+            raise _lib.SpecVerifyError(-4, f"tv_w4_linear: a wait on the device ran out (code {code}), tokens are not valid")
         for ev in evs:
             phases["draft_ms"] += ev[0].elapsed_time(ev[1])
             phases["verify_ms"] += ev[1].elapsed_time(ev[2])

@@ -123,7 +123,7 @@ def dequantize_w4(qweight: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
 
 
 def w4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, *, x_scale: Optional[torch.Tensor] = None,
-              out: Optional[torch.Tensor] = None) -> torch.Tensor:
+              out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x @ W.T`` for a 4-bit weight W [N, K] (``tv_w4_linear``).
 
     x [..., K]: the scales' type (bf16 or fp16), or float8_e4m3fn with
@@ -131,7 +131,9 @@ def w4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, *, x
     returns them; unit stride on K.  qweight [N, K / 8] int32 and scales
     [N, K / group] as :func:`quantize_w4` lays them out (group a multiple of
     32).  Returns [..., N] in the scales' type, summed in fp32; ``out``, when
-    given, is [rows, N] with unit stride on N.
+    given, is [rows, N] with unit stride on N.  ``status`` (int32 [1], zeroed by
+    the caller) receives a nonzero code if a bounded wait on the device ran out;
+    the outputs it concerns are NaN.
     """
     n, words = qweight.shape if qweight.dim() == 2 else (0, 0)
     k, fp8 = words * 8, x.dtype is torch.float8_e4m3fn
@@ -140,8 +142,9 @@ def w4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, *, x
             and scales.shape[0] == n > 1 and qweight.dtype is torch.int32 and scales.dtype in _HALF
             and qweight.stride()[1] == 1 and scales.stride()[1] == 1 and (x.dtype is scales.dtype if not fp8 else False)
             and x_scale is None and out is None and groups and k % (32 * groups) == 0
+            and (status is None or (status.dtype is torch.int32 and status.numel() == 1 and status.device == x.device))
             and x.device == qweight.device == scales.device):
-        _check_w4_linear(x, qweight, scales, x_scale, out)
+        _check_w4_linear(x, qweight, scales, x_scale, out, status)
     x2 = x if x.dim() == 2 else x.reshape(-1, k)
     rows = x2.shape[0]
     if out is None:
@@ -153,6 +156,8 @@ def w4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, *, x
     a = _lib.W4Args(_lib.TV_E4M3 if fp8 else kind, kind, rows, n, k, k // groups, x2.data_ptr(), x2.stride(0),
                     x_scale.data_ptr() if fp8 else None, qweight.data_ptr(), qweight.stride(0) if n > 1 else words,
                     scales.data_ptr(), scales.stride(0), res.data_ptr(), o_sm)
+    if status is not None:
+        a.status = status.data_ptr()
     lib = _lib.load()
     st = _lib.launch(x.device, lib.tv_w4_linear, a)
     if st == _lib.TV_ERR_WORKSPACE:      # rows that have to be laid out anew first; nothing was launched
@@ -167,8 +172,10 @@ def w4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, *, x
     return res
 
 
-def _check_w4_linear(x, qweight, scales, x_scale, out) -> None:
-    _lib.require_cuda(x, qweight, scales, x_scale, out)
+def _check_w4_linear(x, qweight, scales, x_scale, out, status) -> None:
+    _lib.require_cuda(x, qweight, scales, x_scale, out, status)
+    if status is not None and (status.dtype != torch.int32 or status.numel() != 1):
+        raise _lib.SpecVerifyError(-2, f"status must be one int32, got {tuple(status.shape)} {status.dtype}")
     if x.dim() < 1 or qweight.dim() != 2 or scales.dim() != 2 or qweight.shape[0] != scales.shape[0]:
         raise _lib.SpecVerifyError(-1, f"x {tuple(x.shape)}, qweight {tuple(qweight.shape)}, scales "
                                        f"{tuple(scales.shape)}")
