@@ -311,8 +311,10 @@ class PagedKVCache:
         """
         if seq_id not in self.page_tables:
             raise ValueError(f"Sequence {seq_id} not allocated")
+        result = acc.single()
         if path is None:
-            path = acc.to_host()["path"]
+            host = acc.to_host()
+            path = (host[0] if isinstance(host, list) else host)["path"]
         table = self.page_tables[seq_id]
         length = max(max(table.keys()) + 1 if table else 0, (start + len(path)) // self.page_size + 1,
                      (start + max(path)) // self.page_size + 1 if path else 0)
@@ -327,7 +329,7 @@ class PagedKVCache:
         st = _lib.load().tv_compact_paged(
             pool.data_ptr(), self.num_layers * 2, self.num_heads, pool.stride(1) * es, pool.stride(2) * es,
             pool.stride(3) * es, pool.stride(4) * es, self.head_dim * es, self.page_size, src.data_ptr(),
-            dst.data_ptr(), length, self.max_pages, int(start), acc.result.data_ptr(), max(len(path), 1),
+            dst.data_ptr(), length, self.max_pages, int(start), result.data_ptr(), max(len(path), 1),
             _lib.stream_ptr(pool.device))
         _lib.check(st, "tv_compact_paged")
         return start + len(path)

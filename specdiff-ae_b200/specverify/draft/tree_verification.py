@@ -100,6 +100,13 @@ class AcceptResult:
         """Sequence ``b`` of a batched result (:func:`accept_residual`)."""
         return AcceptResult(self.next_tokens[b], self.result[b], self.rows)
 
+    def single(self) -> torch.Tensor:
+        """``result`` as the compaction kernels read it: one sequence's."""
+        if self.result.dim() != 1 and self.result.shape[0] != 1:
+            raise _lib.SpecVerifyError(-1, f"the result of {self.result.shape[0]} sequences: compact them one by one, "
+                                           "with acc.sequence(b)")
+        return self.result
+
     def to_host(self):
         """One D2H copy; returns a dict with python ints / lists (a list of
         them, one per sequence, for a batched result)."""
@@ -338,9 +345,11 @@ def compact_kv(past_key_values_data: List[torch.Tensor], start: int, acc: Accept
 
     Each buffer is ``[..., S_budget, D]`` with the last two dims addressable as
     rows (the reference's ``[2L, B, H_kv, S_budget, D]``).  n and the path come
-    from ``acc`` on the device.  ``tree_verification.py:197-217``.
+    from ``acc`` on the device, one sequence's (``acc.sequence(b)`` of a batch).
+    ``tree_verification.py:197-217``.
     """
     lib = _lib.load()
+    result = acc.single()
     max_rows = acc.rows if max_rows is None else max_rows
     for data in past_key_values_data:
         _lib.require_cuda(data)
@@ -352,7 +361,7 @@ def compact_kv(past_key_values_data: List[torch.Tensor], start: int, acc: Accept
             raise _lib.SpecVerifyError(-3, "KV buffer leading dims must be collapsible")
         es = data.element_size()
         st = lib.tv_compact_contig(flat.data_ptr(), flat.shape[0], flat.stride(0) * es, flat.stride(1) * es,
-                                   flat.shape[2] * es, int(start), acc.result.data_ptr(), int(max_rows),
+                                   flat.shape[2] * es, int(start), result.data_ptr(), int(max_rows),
                                    _lib.stream_ptr(data.device))
         _lib.check(st, "tv_compact_contig")
 

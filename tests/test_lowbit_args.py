@@ -137,3 +137,54 @@ def test_structs_match_the_header(tmp_path):
                    check=True)
     out = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout
     assert [int(x) for x in out.split()] == want
+
+
+def test_compaction_takes_one_sequence(lib):
+    """A batched result would have every slice moved along its first sequence's path."""
+    from specverify.core.kv_cache.paged_kv import PagedKVCache, PagedKVConfig
+    from specverify.draft import AcceptResult, compact_kv
+    both = AcceptResult(torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 14, dtype=torch.int64), 3)
+    with pytest.raises(SpecVerifyError) as e:
+        compact_kv([], 0, both)
+    assert e.value.status == -1
+    compact_kv([], 0, both.sequence(1))
+    compact_kv([], 0, AcceptResult(both.next_tokens[:1], both.result[:1], 3))
+    cache = PagedKVCache(PagedKVConfig(page_size=4, max_pages=4, num_layers=1, num_heads=1, head_dim=8, device="cpu"))
+    cache.allocate_sequence(0, 8)
+    for path in (None, [0, 2]):
+        with pytest.raises(SpecVerifyError) as e:
+            cache.compact_path(0, 2, both, path=path)
+        assert e.value.status == -1
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA device")
+def test_compaction_of_each_sequence_of_a_batch():
+    from specverify.core.kv_cache.paged_kv import PagedKVCache, PagedKVConfig
+    from specverify.draft import accept_residual, compact_kv
+    from specverify.draft.tree_verification import AcceptResult
+    logits = torch.full((2, 4, 50), -30.0, device="cuda")
+    logits[0, 0, 7] = logits[0, 2, 9] = logits[1, 0, 8] = logits[1, 1, 3] = 30.0
+    draft = torch.tensor([[0, 1, 7, 9], [0, 8, 5, 3]], device="cuda")
+    parent = torch.tensor([[-1, -1, 1], [-1, -1, 0]], device="cuda")
+    acc = accept_residual(logits, draft, parent, torch.full((2, 4), 0.5, device="cuda"))
+    paths = [h["path"] for h in acc.to_host()]
+    assert paths == [[0, 2, 3], [0, 1, 3]]
+    kv = torch.randn(2, 3, 20, 64, device="cuda").bfloat16()            # [batch, heads, rows, head_dim]
+    want = kv.clone()
+    for b, path in enumerate(paths):
+        want[b, :, 10:13] = kv[b][:, [10 + i for i in path]]
+    for b in range(2):
+        compact_kv([kv[b]], 10, acc.sequence(b))
+    assert torch.equal(kv, want)
+    # a batch of one is one sequence, in the paged cache too
+    one = AcceptResult(acc.next_tokens[1:], acc.result[1:], 4)
+    caches = []
+    for a, path in ((one, None), (acc.sequence(1), paths[1])):
+        cache = PagedKVCache(PagedKVConfig(page_size=4, max_pages=8, num_layers=1, num_heads=1, head_dim=64,
+                                           dtype=torch.bfloat16, device="cuda"))
+        cache.allocate_sequence(0, 16)
+        cache.page_pool.copy_(torch.randn(cache.page_pool.shape, generator=torch.Generator().manual_seed(1)))
+        assert cache.compact_path(0, 10, a, path=path) == 13
+        caches.append(cache.page_pool)
+    assert torch.equal(*caches)
