@@ -246,6 +246,12 @@ def launch(dev: torch.device, fn, *args) -> int:
         return fn(*args, stream)
 
 
+def fit_i32(what: str, *sizes: int) -> None:
+    """Refuse sizes that the C ABI's 32-bit fields would hold cut off."""
+    if max(sizes) > 0x7FFFFFFF:
+        raise SpecVerifyError(-7, f"{what}: sizes {sizes} have to be below 2^31")
+
+
 def ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 

@@ -230,6 +230,7 @@ def accept_residual(logits: torch.Tensor, draft: torch.Tensor, parent: torch.Ten
                                     and counts.device == logits.device))
             and logits.device == draft.device == parent.device == uniform.device):
         _check_accept_residual(logits, draft, parent, uniform, draft_probs, counts)
+    _lib.fit_i32("tv_residual_accept", b, m, v)
     code = _LOGITS[logits.dtype]
     nxt = draft.new_empty(own + (m,))
     res = draft.new_empty(own + (RESULT_HEADER + 2 * m,))

@@ -52,6 +52,7 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, 
             and residual_out is None):
         _check_add_rms_norm(x, residual, weight, residual_out)
     rows, cols = shape
+    _lib.fit_i32("tv_add_rms_norm", rows, cols)
     h = torch.empty_like(x, memory_format=torch.contiguous_format) if residual_out is None else residual_out
     if fp8:
         y = torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format)
@@ -147,6 +148,7 @@ def w4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, *, x
         _check_w4_linear(x, qweight, scales, x_scale, out, status)
     x2 = x if x.dim() == 2 else x.reshape(-1, k)
     rows = x2.shape[0]
+    _lib.fit_i32("tv_w4_linear", rows, n, k)
     if out is None:
         res = scales.new_empty((rows, n) if x.dim() == 2 else x.shape[:-1] + (n,))
         o_sm = n

@@ -169,3 +169,24 @@ def test_offsets_beyond_32_bits():
     a, b = y8[-5:].double() * scale[-5:, None].double(), a8.double() * ascale[:, None].double()
     assert bool(((a - b).abs() <= (2 * 2.0 ** -4 + 2.0 ** -10) * torch.maximum(a.abs(), b.abs())
                  + 2.0 ** -9 * ascale[:, None]).all())
+
+
+def test_sizes_that_32_bits_do_not_hold_are_refused():
+    """The argument blocks' sizes are 32 bits: 2^32 + 4 rows would be taken as four and the rest left unwritten."""
+    from specverify import SpecVerifyError
+    from specverify.draft import accept_residual
+    from specverify.runtime import add_rms_norm, w4_linear
+    for rows in (2 ** 31, 2 ** 32 + 4):
+        one = torch.ones(1, 1, dtype=torch.bfloat16, device="cuda")
+        x, q, s = problem(1, 2, 32, 32, torch.bfloat16)
+        calls = [lambda: add_rms_norm(one.expand(rows, 1), one.expand(rows, 1), one[0], 1e-5),
+                 lambda: w4_linear(x.expand(rows, 32), q, s),
+                 lambda: w4_linear(x.expand(rows, 1, 32), q, s),
+                 lambda: accept_residual(torch.zeros(1, 1, 4, device="cuda").expand(rows, 1, 4),
+                                         torch.zeros(1, 1, dtype=torch.int64, device="cuda").expand(rows, 1),
+                                         torch.zeros(1, 0, dtype=torch.int64, device="cuda").expand(rows, 0),
+                                         torch.zeros(1, 1, device="cuda").expand(rows, 1))]
+        for call in calls:
+            with pytest.raises(SpecVerifyError) as e:
+                call()
+            assert e.value.status == -7
