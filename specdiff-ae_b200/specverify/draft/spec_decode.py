@@ -438,6 +438,7 @@ class SpecDecodeModel:
         verify, accept (``acceptance`` "match" or, at a temperature, "residual"),
         compact.  Returns (accept result, features of the tree
         rows [M, 3 H], CUDA events around the phases)."""
+        self._check_acceptance(acceptance, temperature)
         ev = [torch.cuda.Event(enable_timing=True) for _ in range(4)]
         ev[0].record()
         if tree is None:
@@ -462,6 +463,13 @@ class SpecDecodeModel:
         self._compact(start, acc, ids.numel())
         ev[3].record()
         return acc, feats, ev
+
+    @staticmethod
+    def _check_acceptance(acceptance: str, temperature: float) -> None:
+        if acceptance not in ("match", "residual"):
+            raise ValueError(f"acceptance {acceptance!r} must be 'match' or 'residual'")
+        if acceptance == "residual" and not temperature > 0:
+            raise ValueError("the residual rule samples: it needs a temperature above 0")
 
     def _uniform(self, n: int, seed: int, offset: int) -> torch.Tensor:
         """Step ``offset``'s uniform numbers: Philox keyed by all 64 bits of
@@ -523,10 +531,7 @@ class SpecDecodeModel:
             raise ValueError("nodes must be a multiple of max_depth")
         if prompt_len + max_new_tokens + nodes + 2 > self.max_tokens:
             raise ValueError("cache too small for the request")
-        if acceptance not in ("match", "residual"):
-            raise ValueError(f"acceptance {acceptance!r} must be 'match' or 'residual'")
-        if acceptance == "residual" and not temperature > 0:
-            raise ValueError("the residual rule samples: it needs a temperature above 0")
+        self._check_acceptance(acceptance, temperature)
         root_tok = self.fill_context(prompt_len, seed)
         root = torch.tensor([root_tok], device=self.device)
         root_feat = torch.zeros((1, 3 * self.shape.hidden), device=self.device, dtype=self.dtype)

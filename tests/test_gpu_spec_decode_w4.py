@@ -171,3 +171,15 @@ def test_residual_rule_draws_other_numbers_for_every_seed_and_step(monkeypatch):
     for i in range(len(runs)):
         for j in range(i):
             assert not set(seen[i]) & set(seen[j]), (runs[i], runs[j])
+
+
+def test_a_step_refuses_an_acceptance_that_it_does_not_know():
+    m = _model()
+    root = m.fill_context(PROMPT, seed=5)
+    before = m.pool.clone()
+    for kw in (dict(acceptance="residua", temperature=1.0), dict(acceptance="residual", temperature=0.0)):
+        with pytest.raises(ValueError):
+            m.step(torch.tensor([root], device="cuda"), torch.zeros(1, 3 * 512, device="cuda", dtype=m.dtype), PROMPT, 2,
+                   4, seed=0, offset=0, **kw)
+    # refused before anything ran; bitwise, as rows that nothing has written yet may hold NaNs
+    assert torch.equal(m.pool.view(torch.int16), before.view(torch.int16))
