@@ -183,3 +183,40 @@ def test_a_step_refuses_an_acceptance_that_it_does_not_know():
                    4, seed=0, offset=0, **kw)
     # refused before anything ran; bitwise, as rows that nothing has written yet may hold NaNs
     assert torch.equal(m.pool.view(torch.int16), before.view(torch.int16))
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+def test_residual_rule_moves_the_accepted_rows_of_every_layer(bits):
+    """The cache after a step, row by row: the accepted path's rows lie behind the context in order, in the K and V of
+    every layer, bitwise as the verify step wrote them at the tree's rows."""
+    from specverify.runtime.draft_tree import finalize_tree
+    m = _model(bits=bits)
+    root = m.fill_context(PROMPT, seed=5)
+    first = _plain_greedy(m, root, PROMPT, 1)[0][0]
+    # two children of the root, the second the target's own token: the path skips a row
+    other = (first + 1) % m.shape.vocab
+    tree = finalize_tree(torch.arange(2, device="cuda"), torch.zeros(1, 2, dtype=torch.int64, device="cuda"),
+                         torch.tensor([[other, first]], device="cuda"), 1, 2, validate=True)
+    m.fill_context(PROMPT, seed=5)
+    state, compact = {}, m._compact
+
+    def watch(start, acc, rows):
+        state["before"] = _rows(m, start, rows)
+        compact(start, acc, rows)
+        state["after"] = _rows(m, start, rows)
+    m._compact = watch
+    acc, _, _ = m.step(torch.tensor([root], device="cuda"), torch.zeros(1, 3 * 512, device="cuda", dtype=m.dtype), PROMPT,
+                       2, 1, 1e-4, 0, 0, tree=tree, acceptance="residual")
+    path = acc.to_host()["path"]
+    assert path == [0, 2]
+    want = state["before"].clone()
+    want[..., :2, :] = state["before"][..., path, :]
+    assert not torch.equal(state["before"][..., 1, :], state["before"][..., 2, :])
+    assert torch.equal(state["after"], want)
+
+
+def _rows(m, start, rows):
+    """K and V of logical rows start .. start + rows of every layer, [layers, 2, kv heads, rows, head_dim]."""
+    pos = torch.arange(start, start + rows, device="cuda")
+    page = m.page_table.view(-1)[pos // m.page].long()
+    return m.pool[:, :, page, :, pos % m.page, :].permute(1, 2, 3, 0, 4).clone()
