@@ -602,10 +602,12 @@ int tv_add_rms_norm(const void* x, int64_t x_row_stride, const void* residual, i
  * scales [n][k / group], row stride s_sn; group a multiple of 32, k a multiple
  * of group.  x [rows][k] (row stride x_sm): out_dtype (bf16 or fp16, also the
  * scales' type), or TV_E4M3 with x_scale [rows] fp32 (NULL otherwise).
- * out [rows][n], row stride o_sm.  Each (u - 8) * s is rounded once to the 16-bit
- * type, sums are in fp32 in an order that sizes fix.  rows == 0 does nothing.
+ * out [rows][n], row stride o_sm; out overlaps no input.  Each (u - 8) * s is
+ * rounded once to the 16-bit type, at every number of rows, sums are in fp32 in an
+ * order that sizes fix.  rows == 0 does nothing.
  * Scales: bf16 of magnitude 2^-80 to 2^30, fp16 up to 8188 (8 s must be finite),
- * or 0.  k <= 2^20, n <= 2^27, rows <= 65535 * 128 (TV_ERR_UNSUPPORTED beyond).
+ * or 0.  Sums in bf16 keep fp32's precision down to magnitudes of 2^-86 (before
+ * x_scale).  k <= 2^20, n <= 2^27, rows <= 65535 * 128 (TV_ERR_UNSUPPORTED beyond).
  * workspace: tv_w4_workspace_size bytes, 16-byte aligned; 0 bytes unless x has to
  * be laid out anew first (more rows than 8, or than fit shared memory, in e4m3,
  * off the 16-byte grid or with k no multiple of 64).  Without one such a call

@@ -21,7 +21,9 @@
 // added in rank order, so results do not depend on timing.
 //
 // Each (u - 8) * s is rounded once to x's 16-bit type (the MMA takes no other):
-// half a step, as the weight itself had in that type.
+// half a step, as the weight itself had in that type.  The error against 64
+// bits is 0.0022 in bf16 and 0.00028 in fp16 with it, 0.0017 and 0.00021 for an
+// unrounded weight (the output's own rounding).
 //
 // What bounds it: an MMA of 128 rows x 16 k takes about 37 cycles however few
 // the tokens (its A operand's way out of tensor memory), so a stage is 0.32 us of

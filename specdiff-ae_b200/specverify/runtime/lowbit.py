@@ -96,6 +96,8 @@ def quantize_w4(weight: torch.Tensor, group: int = 128) -> Tuple[torch.Tensor, t
     ``q = round(w / scale)`` in -8 .. 7.  Returns ``(qweight, scales)``: int32
     [N, K / 8] (layout at ``tv_w4_linear``) and [N, K / group].  Plain torch
     operations on the weight's device, done once when a model is loaded.
+    :func:`w4_linear` takes scales of 2^-80 to 2^30 in bf16 (weights of 2^-78 to
+    2^32 as a group's largest) and up to 8188 in fp16, or 0.
     """
     if weight.dim() != 2 or weight.dtype not in _HALF:
         raise _lib.SpecVerifyError(-1, f"weight must be [N, K] in bfloat16 or float16, got {tuple(weight.shape)} "
@@ -125,14 +127,15 @@ def dequantize_w4(qweight: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
 
 def w4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, *, x_scale: Optional[torch.Tensor] = None,
               out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """``x @ W.T`` for a 4-bit weight W [N, K] (``tv_w4_linear``).
+    """``x @ W.T`` for a 4-bit weight W [N, K] (``tv_w4_linear``), W as
+    :func:`dequantize_w4` has it, rounded to the scales' type.
 
     x [..., K]: the scales' type (bf16 or fp16), or float8_e4m3fn with
     ``x_scale`` (fp32, one per row, shape [...]) as :func:`add_rms_norm`
     returns them; unit stride on K.  qweight [N, K / 8] int32 and scales
     [N, K / group] as :func:`quantize_w4` lays them out (group a multiple of
     32).  Returns [..., N] in the scales' type, summed in fp32; ``out``, when
-    given, is [rows, N] with unit stride on N.  ``status`` (int32 [1], zeroed by
+    given, is [rows, N] with unit stride on N and overlaps no input.  ``status`` (int32 [1], zeroed by
     the caller) receives a nonzero code if a bounded wait on the device ran out;
     the outputs it concerns are NaN.
     """

@@ -229,3 +229,60 @@ def test_refusals():
     for a, b, c, kw in bad:
         with pytest.raises(SpecVerifyError):
             w4_linear(a, b, c, **kw)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,k,group", [(40, 128, 128), (333, 384, 32), (100, 768, 256), (2500, 2048, 128), (48, 4224, 64)])
+def test_every_number_of_rows_multiplies_the_same_weights(n, k, group, dtype):
+    """A token decoded alone, in a frontier and in a tree sees one model: the weights are those of dequantize_w4, rounded
+    once to the 16-bit type, in both kernels.  A row of x with 1 at one k and -1 at another reads the difference of two
+    of them; both have at most 11 bits and lie within 2^9 of each other (or are 0), so that it fits fp32's 24 bits and
+    is rounded once, to the output."""
+    from specverify.runtime import dequantize_w4, w4_linear
+    _, q, s = problem(1, n, k, group, dtype, seed=n + k)
+    w = dequantize_w4(q, s).double()
+    for t in (1, 3, 8, 9, 65, 130):
+        g = torch.Generator().manual_seed(t)
+        a, b = torch.randint(0, k, (2, t), generator=g)
+        b = torch.where(a == b, (b + 1) % k, b)
+        b[0] = a[0] ^ 1                             # one pair in one group
+        x = torch.zeros(t, k)
+        x[torch.arange(t), a] = 1
+        x[torch.arange(t), b] = -1
+        x = x.cuda()
+        want = (w[:, a.cuda()] - w[:, b.cuda()]).t()
+        assert torch.equal(want.float().double(), want)
+        assert torch.equal(w4_linear(x.to(dtype), q, s), want.float().to(dtype)), t
+        xs = torch.full((t,), 0.25, device="cuda")
+        assert torch.equal(w4_linear(x.to(torch.float8_e4m3fn), q, s, x_scale=xs), (want / 4).float().to(dtype)), t
+
+
+# widths of decoders that are no multiple of 2048 along k, groups of 128; one token, a frontier, a tree
+@pytest.mark.parametrize("t", [1, 8, 65])
+@pytest.mark.parametrize("n,k", [(5120, 5120), (4096, 11008), (3584, 2560), (18944, 3584), (1024, 13824)])
+def test_decoder_widths(t, n, k):
+    from specverify.runtime import w4_linear
+    x, q, s = problem(t, n, k, 128, torch.bfloat16, seed=t + k)
+    check(w4_linear(x, q, s), x, q, s)
+    x8, xs = to_fp8(x)
+    check(w4_linear(x8, q, s, x_scale=xs), x8, q, s, xs)
+
+
+@pytest.mark.parametrize("t,n,k,group", [(130, 300, 512, 128), (257, 4099, 1056, 32), (600, 1000, 2048, 64)])
+def test_8_bit_rows_of_a_prompt(t, n, k, group):
+    from specverify.runtime import w4_linear
+    x, q, s = problem(t, n, k, group, torch.float16, seed=t)
+    x8, xs = to_fp8(x)
+    check(w4_linear(x8, q, s, x_scale=xs), x8, q, s, xs)
+
+
+@pytest.mark.parametrize("t", [3, 20])
+@pytest.mark.parametrize("value", [2.0 ** -60, 2.0 ** 110])
+def test_small_and_large_rows(t, value):
+    """bf16 sums are held times 2^-40; far from 1 they keep fp32's precision all the same (products here of 2^-70 and
+    2^-10 times 2^110)."""
+    from specverify.runtime import w4_linear
+    _, q, s = problem(t, 200, 512, 128, torch.bfloat16, seed=8)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = (value * torch.randn(t, 512, device="cuda", generator=g)).to(torch.bfloat16)
+    check(w4_linear(x, q, s), x, q, s)
