@@ -584,7 +584,7 @@ int tv_silu_mul(const void* gate, const void* up, int64_t in_row_stride, void* o
  *     f = h * inv * weight in fp32, y_scale[r] = max|f| / 448,
  *     y = e4m3(f / y_scale[r]).  A row of zeros has scale 0; a row with a NaN
  *     has scale NaN and NaN throughout.
- * Any cols >= 1, strides and alignment (rows of 16-byte multiples at 16-byte
+ * cols from 1 to 2^30 (TV_ERR_UNSUPPORTED beyond), any strides and alignment (rows of 16-byte multiples at 16-byte
  * aligned addresses are read as vectors).  rows == 0 does nothing. */
 int tv_add_rms_norm(const void* x, int64_t x_row_stride, const void* residual, int64_t residual_row_stride,
                     const void* weight, void* residual_out, int64_t residual_out_row_stride, void* y,

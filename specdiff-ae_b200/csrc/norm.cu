@@ -391,6 +391,7 @@ int tv_add_rms_norm(const void* x, int64_t x_row_stride, const void* residual, i
                     void* stream) {
   if (rows < 0 || cols <= 0) return TV_ERR_SHAPE;
   if (dtype != TV_BF16 && dtype != TV_F16) return TV_ERR_DTYPE;
+  if (cols > (1 << 30)) return TV_ERR_UNSUPPORTED;      // a thread's column index passes cols by up to 4096
   if (rows == 0) return TV_OK;
   if (!x || !residual || !weight || !residual_out || !y) return TV_ERR_NULL;
   AddNormArgs a{x, residual, weight, residual_out, y, y_scale, x_row_stride, residual_row_stride,

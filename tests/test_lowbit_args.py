@@ -157,6 +157,15 @@ def test_compaction_takes_one_sequence(lib):
         assert e.value.status == -1
 
 
+def test_add_rms_norm_refuses_rows_that_its_column_index_does_not_hold(lib):
+    """A thread steps over a wide row 4096 columns at a time in 32 bits: behind 2^31 - 4096 the index would turn negative."""
+    for cols in (2 ** 31 - 1, 2 ** 31 - 4096, 2 ** 30 + 1):
+        for y_scale in (None, FAKE):
+            assert lib.tv_add_rms_norm(FAKE, cols, FAKE, cols, FAKE, FAKE, cols, FAKE, cols, y_scale, 0, cols, 1e-5, 0,
+                                       None) == -7
+    assert lib.tv_add_rms_norm(FAKE, 8, FAKE, 8, FAKE, FAKE, 8, FAKE, 8, None, 0, 2 ** 30, 1e-5, 0, None) == 0
+
+
 @pytest.mark.gpu
 @pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA device")
 def test_compaction_of_each_sequence_of_a_batch():
