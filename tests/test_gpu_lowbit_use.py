@@ -190,3 +190,79 @@ def test_sizes_that_32_bits_do_not_hold_are_refused():
             with pytest.raises(SpecVerifyError) as e:
                 call()
             assert e.value.status == -7
+
+
+def test_captured_behind_copies_memsets_and_a_fork():
+    """Launches that may start while their predecessor ends, captured where that predecessor is a copy, a memset, two
+    kernels on different streams that meet, or one that takes its time."""
+    from specverify.draft import accept_residual
+    from specverify.runtime import add_rms_norm, w4_linear
+    x, q, s = problem(65, 4096, 2048, 128, torch.bfloat16, seed=21)
+    few, fq, fs = problem(2, 2048, 2048, 128, torch.bfloat16, seed=22)
+    w = torch.rand(2048, device="cuda").bfloat16()
+    r = torch.zeros_like(x)
+    stage, sums = torch.zeros_like(x), torch.zeros_like(x)
+    draft = torch.randint(0, 4096, (65,), device="cuda")
+    parent = torch.arange(-1, 63, device="cuda") // 2
+    u = torch.rand(65, device="cuda")
+    big = torch.randn(4096, 4096, device="cuda")
+
+    def run(side):
+        slow = (big @ big)[0, 0] * 0                  # some hundred microseconds
+        stage.copy_(x)                                # a memory copy
+        sums.zero_()                                  # a memset
+        y, h = add_rms_norm(stage, sums, w, 1e-5)
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            z = w4_linear(few + slow.bfloat16(), fq, fs)          # a join of two streams in front of the norm
+        logits = w4_linear(y, q, s)
+        here.wait_stream(side)
+        r[:2] = z
+        y8, scale, h2 = add_rms_norm(h, r, w, 1e-5, fp8=True)
+        logits2 = w4_linear(y8, q, s, x_scale=scale)
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            a = accept_residual(logits, draft, parent, u)
+        b = accept_residual(logits2, draft, parent, u)
+        here.wait_stream(side)
+        return y, h, logits, z, y8.view(torch.uint8), scale, h2, logits2, a.result, b.result
+
+    torch.cuda.synchronize()
+    want = [t.clone() for t in run(torch.cuda.Stream())]
+    torch.cuda.synchronize()
+    y, h, logits = want[:3]
+    check(logits, y, q, s)
+    check(want[3], few, fq, fs)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(torch.cuda.Stream())
+    for _ in range(5):
+        for t in out:
+            t.zero_()
+        r.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_calls_from_several_threads():
+    import threading
+    runs = [chain(5), chain(6, 9), chain(7, 3), chain(8, 130)]
+    want = [[t.clone() for t in run()] for run in runs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                out = runs[i]()
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(out, want[i])):
+                    bad.append(i)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
