@@ -25,11 +25,16 @@ inline int check_launch() {
 
 // ---- kernels that start while the one before them ends ----------------------
 // A kernel launched by launch_early may start once every CTA of its predecessor
-// in the stream has called grid_next or ended; before it touches global memory
-// it calls grid_wait, which returns when the predecessor has completed and its
-// writes are visible.  What comes before that (the launch itself, barriers,
-// tensor memory) is off the critical path.  Every such kernel waits, so
-// completion carries over a chain of them.
+// in the stream has called grid_next or ended; before it reads or writes global
+// memory it calls grid_wait, which returns when the predecessor has completed and
+// its writes are visible.  What comes before that (the launch itself, barriers,
+// requests that only bring lines to L2) is off the critical path.  Every such
+// kernel waits, so completion carries over a chain of them.
+//
+// One kernel reads before its wait: the residual rule's second stage, what its
+// first stage does not write (the tree, the uniform numbers, drafted words'
+// logits).  That is safe only behind a first stage that calls grid_next AFTER its
+// own grid_wait, where whatever wrote those inputs has completed.
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -347,11 +347,10 @@ int pick_add_norm(const AddNormArgs& a, int rows, AddNormLayout layout, cudaStre
     if (fit(1) <= 512 && !(many && chunks >= 128)) return launch_add_norm<T, FP8, 8, 1, false, true>(a, rows, fit(1), st);
     if (fit(4) <= 512) return launch_add_norm<T, FP8, 8, 4, false, true>(a, rows, fit(4), st);
   }
-  if (layout == kRowsAny || layout == kRowsShifted) {
-    const int t = (a.cols + 15) / 16 / 32 * 32 + 32;
-    if (a.cols <= 2048) return launch_add_norm<T, FP8, 1, 4, false, false>(a, rows, ((a.cols + 3) / 4 + 31) / 32 * 32, st);
-    if (t <= 512) return launch_add_norm<T, FP8, 1, 16, false, false>(a, rows, t, st);
-  }
+  // element by element
+  const int t = (a.cols + 15) / 16 / 32 * 32 + 32;
+  if (a.cols <= 2048) return launch_add_norm<T, FP8, 1, 4, false, false>(a, rows, ((a.cols + 3) / 4 + 31) / 32 * 32, st);
+  if (t <= 512) return launch_add_norm<T, FP8, 1, 16, false, false>(a, rows, t, st);
   return launch_add_norm<T, FP8, 1, 1, true, false>(a, rows, 512, st);
 }
 

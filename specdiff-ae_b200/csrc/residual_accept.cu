@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(kStatThreads) row_stats_kernel(const Args a) {
   constexpr int VEC = 16 / sizeof(E);
   constexpr int U = kChunkBytes / (16 * kStatThreads);
   grid_wait();
-  grid_next();        // not before: stage 2 reads the tree without a wait of its own
+  grid_next();        // not before: stage 2 reads its inputs ahead of its own wait
   const int row = blockIdx.y, b = blockIdx.z;
   if (a.counts && row >= a.counts[b]) return;
   const int lo = blockIdx.x * a.chunk;
@@ -298,7 +298,8 @@ __global__ void __launch_bounds__(kWalkThreads, 1) walk_kernel(const Args a) {
   }
   __syncthreads();
   const bool bad = sh.status != TV_OK;
-  // the drafted words' logits and the draw's number, on their way while stage 1 ends
+  // the drafted words' logits and the draw's number, on their way while stage 1
+  // ends; like the tree above they come before this kernel's grid_wait, behind stage 1's
   const float u0 = n > 0 ? u[0] : 0.f;
   float child_logit[2];
 #pragma unroll
