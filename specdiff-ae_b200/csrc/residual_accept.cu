@@ -37,8 +37,7 @@
 // over the ending row, 2 for the draw, each a few dependent round trips.  32
 // sampled trees of 9 take 62 us, stage 1 19 of them (11.3 at the HBM rate): a pass
 // over 32064 words an SM is 9 us of issue (some 65 instructions a word), and the
-// sequence with the most rejections makes three or four.  Folding the first two
-// passes into one by correcting stage 1's normaliser afterwards took 60.4.
+// sequence with the most rejections makes three or four.
 #include <cooperative_groups.h>
 
 #include <atomic>

@@ -28,10 +28,10 @@
 // What bounds it: an MMA of 128 rows x 16 k takes about 37 cycles however few
 // the tokens (its A operand's way out of tensor memory), so a stage is 0.32 us of
 // an SM's tensor pipe, and two CTAs there were seen to take 0.37 a stage: 65
-// rows x 28672 x 4096 (21.7 us) spend 12 us in that (16 stages, two CTAs on half
+// rows x 28672 x 4096 (21.8 us) spend 12 us in that (16 stages, two CTAs on half
 // of the SMs, one on the others), the rest on the way to the first weights (2-3)
 // and from the last MMA to the stored rows (2).  128 rows x 128256 x 4096: 119 us,
-// 1.13 PFLOP/s.  Where k is split, 65 rows x 4096 x 14336 take 16.0 us, 4 of them
+// 1.13 PFLOP/s, and 136 once the power cap has the SMs at 1.6 GHz.  Where k is split, 65 rows x 4096 x 14336 take 16.0 us, 4 of them
 // behind the last MMA: two cluster barriers and the sums' way between SMs.
 // Tiles of 256 weight rows with k cut evenly over the SMs balance better and were
 // slower, as were pairs of CTAs splitting k (37 us at 28672 x 4096): partial sums

@@ -21,8 +21,9 @@ template <typename T> __device__ __forceinline__ uint32_t as_bits(T v) { return 
 // 2^30 stay inside the exponent range.  9 instructions for 8 weights; the
 // usual 128 + u form needs a subtraction and a product, 15.
 //
-// fp16's exponents are too few for that: 1024 + u (or 1024 + 16 u), made by
-// OR, loses its offset in one exact operation, then the product rounds once.
+// fp16's exponents are too few for that.  It takes the form that 4-bit kernels
+// commonly have: 1024 + u (or 1024 + 16 u), made by OR, loses its offset in one
+// exact operation, then the product rounds once.
 template <typename T> struct Unpack;
 template <> struct Unpack<__nv_bfloat16> {
   __nv_bfloat162 sa, sb, off;

@@ -26,15 +26,22 @@
 // before this one ends (16.3 -> 15.1 us at one row x 28672 x 4096, 18.0 -> 16.6 at
 // 8); requests further ahead, all along the way, were slower (18.2 and 19.7).
 //
-// One row x 28672 x 4096 takes 15.1 us, 8 rows 16.6 (9.0 at the measured HBM
-// rate): issue comes next to HBM, about 140 instructions a warp for 2048 weights,
-// 72 of them the unpacking, 5.7 us of every scheduler.  Before the bulk requests:
-// two CTAs of eight warps an SM, up to 16 units on one SM and 8 on another, took
-// 18.8 and 21.7 where this form took 17.2 and 18.4; one batch of four blocks in
-// flight instead of two 19.2 and 20.3.  Whole units a warp (no split of k) took 18.9
-// at 8 x 28672 x 4096, but 10.4 for 7.7 at 8 x 6144 x 4096; teams of eight 19.5 and
-// 8.1.  16 rows (two tiles of N) took 10.2 for the tcgen05 kernel's 10.5 at 6144 x
-// 4096 and 26.1 for 22.4 at 28672 x 4096, so that takes over at 9.
+// One row x 28672 x 4096 takes 15.1 us, 8 rows 16.6 (9.3 at the measured HBM
+// rate), and no pipe is at its limit: about 140 instructions a warp for 2048
+// weights, 72 of them the unpacking, are 7 us of every scheduler's 16.6, HBM runs
+// at 56 %.  3 us go to the start and the first round trip, the rest to waits for
+// loads that eight blocks in flight do not cover.  The uneven last round is not
+// it: 28416 rows, three units for every team, take 16.1 us.
+//
+// That is with the four scales of a batch in one load: group 128, k a multiple of
+// 2048.  Elsewhere each lane loads the scale of its 32 k by itself: 8 rows x 28672
+// x 4096 take 28.5 us at group 64 and 27.9 at 256, one row x 4096 x 11008 takes
+// 15.4 (10240: 8.0).
+//
+// Whole units a warp (no split of k) took 18.9 us at 8 x 28672 x 4096, but 10.4 for
+// 7.7 at 8 x 6144 x 4096; teams of eight 19.5 and 8.1.  Two tiles of N (16 rows)
+// took 10.2 us for the tcgen05 kernel's 10.5 at 6144 x 4096 and 26.1 for 22.4 at
+// 28672 x 4096 (group 128), so that takes over at 9.
 #include <cuda_fp8.h>
 
 #include <type_traits>
