@@ -337,8 +337,8 @@ int tv_accept(const tv_accept_args* args, void* stream);
  * elsewhere.  A sequence with a bad parent, draft token or count, or whose
  * walk ends at a row that is no distribution (no finite logit, a NaN, +inf),
  * gets result[0] = TV_ERR_INPUT, a path of length 0 and token -1.
- * rows <= 1024.  workspace: tv_residual_accept_workspace_size bytes, 16-byte
- * aligned. */
+ * rows <= 1024, batch <= 65535, vocab <= 2^30 (TV_ERR_UNSUPPORTED beyond).
+ * workspace: tv_residual_accept_workspace_size bytes, 16-byte aligned. */
 typedef struct tv_residual_accept_args {
   int32_t logits_dtype;          /* TV_BF16, TV_F16 or TV_F32               */
   int32_t batch, rows, vocab;

@@ -203,6 +203,7 @@ def accept_residual(logits: torch.Tensor, draft: torch.Tensor, parent: torch.Ten
     draft, ``uniform[0]`` draws the final token.  A batch has a leading
     dimension everywhere; ``counts`` (int32 [B], or [1]) is then each
     sequence's number of nodes, the rest being padding that is not read.
+    M up to 1024, B up to 65535.
 
     ``draft_probs`` None: the drafts are fixed (the draft's top-k); with
     ``draft_probs`` [.., M, V] each node's children were drawn independently

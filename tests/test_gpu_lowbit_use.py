@@ -266,3 +266,69 @@ def test_calls_from_several_threads():
     for t in threads:
         t.join()
     assert not bad
+
+
+@pytest.mark.parametrize("t,n,k,group,fp8", [(1, 130, 2 ** 20, 128, False), (9, 40, 2 ** 20, 32, True),
+                                             (3, 64, 104448 // 3 // 32 * 32, 32, False), (8, 33, 13056, 128, True),
+                                             (8, 33, 13088, 32, False), (1, 2 ** 27, 32, 32, False)])
+def test_products_at_the_ends_of_their_ranges(t, n, k, group, fp8):
+    """The longest k, the most that fits an SM's shared memory and one step more, the most outputs (its last columns
+    and some in between)."""
+    from specverify.runtime import w4_linear
+    x, q, s = problem(t, n, k, group, torch.bfloat16, seed=t)
+    x, xs = to_fp8(x) if fp8 else (x, None)
+    y = w4_linear(x, q, s, x_scale=xs)
+    for lo in sorted({0, n // 2, max(0, n - 500)}):
+        cols = slice(lo, lo + 500)
+        check(y[:, cols].contiguous(), x, q[cols], s[cols], xs)
+
+
+def test_a_very_wide_row():
+    """2^24 + 5 columns off the 16-byte grid, one CTA a row.  A thread adds 2^15 squares one after another: the sum is
+    off by less than 2^15 * 2^-24 of itself and 2^-16 for the rest, its inverse root by half of that."""
+    from specverify.runtime import add_rms_norm
+    cols = 2 ** 24 + 5
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x, r = (torch.randn(2, cols, device="cuda", generator=g).bfloat16() for _ in range(2))
+    w = torch.rand(cols, device="cuda", generator=g).bfloat16()
+    y, h = add_rms_norm(x, r, w, 1e-5)
+    assert torch.equal(h, x + r)
+    f = h.double()
+    want = f / (f.square().mean(1, keepdim=True) + 1e-5).sqrt() * w.double()
+    off = 2.0 ** -10 + 2.0 ** -16
+    assert bool(((y.double() - want).abs() <= want.abs() * ((1 + off) * (1 + 2.0 ** -8) ** 2 - 1) + 2.0 ** -125).all())
+
+
+@pytest.mark.parametrize("b,m,v", [(65535, 2, 5), (2, 1024, 257), (1, 2, 4 * 2 ** 20 + 3)])
+def test_acceptance_at_the_ends_of_its_ranges(b, m, v):
+    """The largest batch and tree, a vocabulary of many blocks a CTA, against the rule on whole tensors in 64 bits:
+    a chain whose drafts are all tried in order (every node has one child)."""
+    from specverify.draft import accept_residual
+    g = torch.Generator(device="cuda").manual_seed(b)
+    logits = torch.randn(b, m, v, device="cuda", generator=g)
+    p = torch.softmax(logits.double(), -1)
+    draft = torch.randint(0, v, (b, m), device="cuda", generator=g)
+    draft[:, 1:] = logits[:, :-1].argmax(-1)                       # drafts with a chance
+    parent = torch.arange(-1, m - 2, device="cuda").expand(b, m - 1).contiguous()
+    u = torch.rand(b, m, device="cuda", generator=g)
+    if m > 100:
+        u[:, 1:m // 2] *= 1e-3                                     # a path of some length
+    acc = accept_residual(logits, draft, parent, u)
+    pt = torch.gather(p[:, :-1], 2, draft[:, 1:, None])[..., 0]
+    ok = u[:, 1:].double() < pt
+    n = ok.long().cumprod(1).sum(1) + 1
+    at = torch.arange(b, device="cuda")
+    rest = p[at, n - 1].clone()
+    has = n < m
+    rest[at[has], draft[at[has], n[has]]] = 0
+    cdf = rest.cumsum(-1)
+    edge = u[:, 0].double() * cdf[:, -1]
+    token = torch.searchsorted(cdf, edge[:, None], right=True)[:, 0].clamp(max=v - 1)
+    # comparisons within 2^-20 of a border (a fp32 normaliser's few roundings, and for the draw far more than the
+    # pairs' error) are left out; they are few
+    near = ((u[:, 1:].double() - pt).abs() < 2.0 ** -20 * pt).any(1)
+    near |= (cdf - edge[:, None]).abs().amin(1) < 2.0 ** -34
+    assert float(near.double().mean()) < 0.01
+    keep = ~near
+    assert (acc.result[:, 0] == 0).all() and bool(keep.any())
+    assert torch.equal(acc.result[keep, 2], n[keep]) and torch.equal(acc.result[keep, 3], token[keep])
